@@ -20,7 +20,10 @@ CSRC = os.path.join(os.path.dirname(PKG_DIR), "csrc")
 INCLUDE = os.path.join(os.path.dirname(os.path.dirname(PKG_DIR)), "include")
 OUT = os.path.join(PKG_DIR, "libitts_hip.so")
 ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950")
-FLAGS = ["-O3", "-std=c++17", "-fPIC", "-Wno-unused-result"]
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32, which hipcc -O3 forms from ordinary float code by itself (the
+# host pass warns that it does not know the feature: harmless)
+FLAGS = ["-O3", "-std=c++17", "-fPIC", "-Wno-unused-result",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def sources():
