@@ -8,7 +8,8 @@
  *     legacy default stream); launches are asynchronous, no host synchronisation;
  *   - return 0 on success, nonzero on an argument error or a HIP launch error; the message is in
  *     itts_last_error() (thread-local); no C++ exception crosses the ABI;
- *   - dtype codes: ITTS_F32 = 0, ITTS_BF16 = 1, ITTS_F16 = 2 (f16: the activation op only);
+ *   - dtype codes: ITTS_F32 = 0, ITTS_BF16 = 1, ITTS_F16 = 2 (f16: the activation op only), ITTS_E4M3 = 3
+ *     (block-scaled 8-bit codes: the 8-bit operators only);
  *   - "channel-last" vocoder activations are [B][T][C] with per-sequence lengths[B] (ragged batch):
  *     rows t >= lengths[b] are never read as data (edge handling equals the reference's padding);
  *   - callable from any host thread; ctypes releases the GIL around every call.
@@ -27,7 +28,7 @@
 extern "C" {
 #endif
 
-enum { ITTS_DTYPE_F32 = 0, ITTS_DTYPE_BF16 = 1, ITTS_DTYPE_F16 = 2 };
+enum { ITTS_DTYPE_F32 = 0, ITTS_DTYPE_BF16 = 1, ITTS_DTYPE_F16 = 2, ITTS_DTYPE_E4M3 = 3 };
 
 /* ---- runtime -------------------------------------------------------------------------------- */
 const char* itts_last_error(void);
@@ -35,7 +36,7 @@ int itts_abi_version(void);
 const char* itts_build_target(void); /* "gfx950" */
 /* sizeof of the ABI structs below (0 ItTsGptLayerW, 1 ItTsGptWeights, 2 ItTsGptDecodeState,
  * 3 ItTsSampling, 4 ItTsConv, 5 ItTsAct, 6 ItTsAmpLayer, 7 ItTsBigvganStage, 8 ItTsBigvganWeights,
- * 9 ItTsGptSeqLayerW, 10 ItTsGptSeqWeights, 11 ItTsGptPlLayerW),
+ * 9 ItTsGptSeqLayerW, 10 ItTsGptSeqWeights, 11 ItTsGptPlLayerW, 12 ItTsKvCache),
  * -1 otherwise: lets a binding check its struct layouts. */
 int64_t itts_struct_size(int which);
 
@@ -512,6 +513,73 @@ int itts_gpt_pl_error(const void* scratch, void* stream, int* code);
  * logits only, nsteps = 1, the caller runs the beam kernels and the step advance) as itts_gpt_decode_step. */
 int itts_gpt_decode_steps_pl(const ItTsGptWeights* w, const ItTsGptPlLayerW* pl, void* scratch,
                              const ItTsGptDecodeState* state, const ItTsSampling* sampling, int nsteps, void* stream);
+
+/* ---- 8-bit operators and attention for drafted tokens -------------------------------------------
+ * No counterpart in the reference (it computes in fp16 / fp32).  Block-scaled e4m3: a block of values shares
+ * one power-of-two scale 2^(byte - 127), each value an OCP e4m3 code.  The scale is the smallest power of two
+ * that brings the block's largest finite magnitude within 448 (byte >= 1; 127 for a block without a nonzero
+ * finite value); codes round to nearest even; what is not finite becomes NaN and does not count for the scale. */
+
+/* Rows x [M][K] f32 or bf16 -> codes q [M][ldq] and scale bytes s [M][lds], one scale per 128 consecutive k.
+ * ldq >= K rounded up to 128 (codes behind K: 0), a multiple of 16; lds >= ceil(K / 128) rounded up to 4
+ * (bytes behind the last block: 127), a multiple of 4; q 16-B, s 4-B aligned.  Weights [N][K] of
+ * itts_fp8_linear are quantised by the same call. */
+int itts_fp8_quant_rows(const void* x, int64_t ldx, int x_dtype, int64_t M, int K, uint8_t* q, int64_t ldq, uint8_t* s,
+                        int64_t lds, void* stream);
+/* y [M][N] = act(Q(x) Q(w)^T + bias) + residual: x [M][K] f32 or bf16 is quantised within the call, w comes
+ * quantised (itts_fp8_quant_rows), bias [N] f32 and residual [M][ldr] f32 optional (residual may be y itself),
+ * act 0 none, 1 gelu_tanh, 2 SiLU (as itts_igemm_fwd), y f32 (exact products, f32 accumulation) or bf16 (the 8-bit
+ * matrix unit: f32 accumulation of 128 products at a time, which it aligns to the largest of them).  A row's result does
+ * not depend on the other rows' values; workspace: itts_fp8_linear_workspace_bytes, 16-B aligned, not shared by
+ * calls that may run at the same time (two captured graphs included). */
+int64_t itts_fp8_linear_workspace_bytes(int64_t M, int N, int K);
+int itts_fp8_linear(const void* x, int64_t ldx, int x_dtype, int64_t M, int K, const uint8_t* wq, int64_t ldw,
+                    const uint8_t* ws, int64_t ldws, int N, const float* bias, int act, const float* residual,
+                    int64_t ldr, void* y, int64_t ldy, int out_dtype, void* workspace, void* stream);
+
+/* A KV cache: dtype ITTS_E4M3: codes k / v [rows][heads][max_kv][head_dim] with one scale byte per position in
+ * k_scale / v_scale [rows][heads][max_kv] (block = the head_dim values of one position); dtype ITTS_BF16: k / v
+ * bf16 in the same order (the decode cache of ItTsGptDecodeState, one layer), scales unused.  bs / hs: elements
+ * from row to row / head to head (sbs / shs: of the scale bytes).  head_dim 64 or 128; 16-B aligned rows. */
+typedef struct ItTsKvCache {
+  void *k, *v;
+  uint8_t *k_scale, *v_scale;
+  int64_t bs, hs, sbs, shs;
+  int rows, heads, max_kv, head_dim, dtype;
+} ItTsKvCache;
+/* Quantise k / v [M][heads][head_dim] (f32 or bf16; token and head strides in elements, unit head_dim stride) into
+ * slots (row[i], pos[i]) of an e4m3 cache.  A slot outside the cache (row or pos < 0, or too large) is skipped;
+ * slots not named keep what they held; the slots of one call must differ from each other.  itts_kv8_read: the same
+ * slots dequantised into k / v (zeros for a slot outside the cache). */
+int itts_kv8_write(const ItTsKvCache* c, const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
+                   int64_t v_sh, int dtype, const int32_t* row, const int32_t* pos, int M, void* stream);
+int itts_kv8_read(const ItTsKvCache* c, const int32_t* row, const int32_t* pos, int M, void* k, int64_t k_st,
+                  int64_t k_sh, void* v, int64_t v_st, int64_t v_sh, int dtype, void* stream);
+/* Workspace bytes of the two calls below (16-B aligned; not shared by calls that may run at the same time), -1 for
+ * sizes that they refuse: B rows, T tokens (1: itts_attn_decode_kv8), `group` query heads per K/V head, max_len as
+ * given to the call. */
+int64_t itts_attn_cached_workspace_bytes(const ItTsKvCache* c, int B, int T, int group, int max_len, int q_dtype);
+/* Single-token attention over an e4m3 cache that holds this step's K/V already (itts_kv8_write):
+ * out[b][hq] = softmax(scale * q[b][hq] . K[p]) V[p] over p in [pad[b], kv_len[b]) of cache row b, hq = 0 ..
+ * heads * group - 1 with K/V head hq / group; 0 where that range is empty.  pad may be NULL (0).  kv_rows
+ * (optional): key p of row b is read from cache row kv_rows[b * ld_rows + p] (the beams' lineage table of
+ * itts_attn_decode_rows); an entry outside the cache makes that row's output NaN.  kv_len outside 0 .. max_kv: NaN.
+ * max_len: the largest kv_len the caller expects (it sizes the split over keys; larger ones stay right).
+ * q f32 or bf16, out bf16 or f32 (strides in elements, unit head_dim stride). */
+int itts_attn_decode_kv8(const ItTsKvCache* c, const void* q, int64_t q_sb, int64_t q_sh, int q_dtype, int B, int group,
+                         const int32_t* kv_len, const int32_t* pad, const int32_t* kv_rows, int64_t ld_rows, float scale,
+                         int max_len, void* out, int64_t o_sb, int64_t o_sh, int out_dtype, void* workspace, void* stream);
+/* Attention of T <= 64 drafted tokens per row, q [B][T][heads * group][head_dim], over a cache (e4m3 or bf16) that
+ * holds their K/V at positions kv_len[b] .. kv_len[b] + n - 1 behind the row's kv_len[b] accepted positions
+ * (n = n_tokens[b], NULL: T).  Token t sees p in [pad[b], kv_len[b]) and the drafted token j wherever bit j of
+ * mask[b * mask_sb + t] is set (its ancestors and itself; any set of bits is allowed, bits >= n are ignored; mask_sb
+ * 0: one tree for all rows).  What a token does not see does not reach it, NaN included; a token that sees nothing
+ * gives 0.  Outputs of tokens >= n are left as they were.  kv_len < 0, n outside 0 .. T or kv_len + n > max_kv: the
+ * row's T outputs are NaN.  The rest as itts_attn_decode_kv8; over a bf16 cache out is bf16. */
+int itts_attn_tree(const ItTsKvCache* c, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int q_dtype, int B,
+                   int T, int group, const int32_t* kv_len, const int32_t* pad, const int32_t* n_tokens,
+                   const uint64_t* mask, int64_t mask_sb, const int32_t* kv_rows, int64_t ld_rows, float scale, int max_len,
+                   void* out, int64_t o_sb, int64_t o_st, int64_t o_sh, int out_dtype, void* workspace, void* stream);
 
 /* ---- diagnostics ------------------------------------------------------------------------------ */
 /* n_wg workgroups that each hold 120 KiB of LDS (one per CU) for `usec` microseconds, then exit (sink: NULL

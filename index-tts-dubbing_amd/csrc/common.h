@@ -13,7 +13,7 @@ typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
 
-enum ItTsDtype { ITTS_F32 = 0, ITTS_BF16 = 1, ITTS_F16 = 2 };
+enum ItTsDtype { ITTS_F32 = 0, ITTS_BF16 = 1, ITTS_F16 = 2, ITTS_E4M3 = 3 };
 
 // ---- bf16 <-> f32 (bf16 carried as raw uint16_t) ----
 __device__ __forceinline__ float bf2f(uint16_t v) { return __uint_as_float(((uint32_t)v) << 16); }
@@ -122,6 +122,8 @@ inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s);
 // mel_head + token selection + next embedding of decode step k (gpt_step.hip)
 int gpt_head_sample(const ItTsGptWeights* w, const ItTsGptDecodeState* st, const ItTsSampling* smp, int k,
                     void* stream);
+// the sizes, strides and alignment of a KV cache (kv8.hip)
+int check_kv_cache(const char* fn, const ItTsKvCache* c);
 }  // namespace itts
 
 #define ITTS_REQUIRE(cond, fn, what) \

@@ -1,0 +1,35 @@
+// Block-scaled e4m3: a block of values shares one power-of-two scale 2^(byte - 127), and each value is held as an
+// OCP e4m3 code (1-4-3, largest 448, one NaN per sign, no infinity).  The scale is the smallest power of two that
+// brings the block's largest finite magnitude within 448, so x / scale is exact (f32 keeps every bit of it) and
+// the codes are defined bit for bit: the rounding to 8 bits is the only one.  Values that are not finite become
+// the NaN code and do not count for the scale; a block without a nonzero finite value has the byte 127.
+#pragma once
+#include "common.h"
+
+namespace itts {
+
+constexpr float kE4m3Max = 448.f;  // 1.75 * 2^8
+
+__device__ __forceinline__ bool finite_f(float x) { return fabsf(x) < __builtin_inff(); }
+
+// scale byte of a block whose largest finite magnitude is a: E = min { e : a <= 1.75 * 2^(8 + e) }, e >= -126
+__device__ __forceinline__ int e4m3_scale_byte(float a) {
+  const uint32_t u = __float_as_uint(a);
+  const int e = (int)(u >> 23) - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  return u == 0 ? 127 : (e < 1 ? 1 : e);
+}
+// 1 / scale, exact: bytes are 1 .. 247
+__device__ __forceinline__ float e4m3_inv_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
+__device__ __forceinline__ float e4m3_scale(int byte) { return __uint_as_float((uint32_t)byte << 23); }
+
+// four codes (round to nearest even) of four values already divided by the scale
+__device__ __forceinline__ uint32_t e4m3_pack4(float a, float b, float c, float d) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+// v * inv, with what is not finite as NaN
+__device__ __forceinline__ float e4m3_prescale(float v, float inv) {
+  return finite_f(v) ? v * inv : __builtin_nanf("");
+}
+
+}  // namespace itts

@@ -33,7 +33,8 @@ extern "C" int itts_abi_version(void) { return 5; }  // 3: persistent decode lay
 extern "C" const char* itts_build_target(void) { return "gfx950"; }
 
 // sizeof of the ABI structs (include/itts_hip.h), so bindings can check their layouts:
-// 0 ItTsGptLayerW, 1 ItTsGptWeights, 2 ItTsGptDecodeState, 3 ItTsSampling, 4-8 the vocoder structs
+// 0 ItTsGptLayerW, 1 ItTsGptWeights, 2 ItTsGptDecodeState, 3 ItTsSampling, 4-8 the vocoder structs,
+// 9-11 the sequence and persistent-layer structs, 12 ItTsKvCache
 extern "C" int64_t itts_struct_size(int which) {
   switch (which) {
     case 0: return sizeof(ItTsGptLayerW);
@@ -48,6 +49,7 @@ extern "C" int64_t itts_struct_size(int which) {
     case 9: return sizeof(ItTsGptSeqLayerW);
     case 10: return sizeof(ItTsGptSeqWeights);
     case 11: return sizeof(ItTsGptPlLayerW);
+    case 12: return sizeof(ItTsKvCache);
     default: return -1;
   }
 }

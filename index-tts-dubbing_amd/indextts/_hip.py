@@ -18,7 +18,7 @@ LIB_NAME = "libitts_hip.so"
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, LIB_NAME)
 
-F32, BF16, F16 = 0, 1, 2
+F32, BF16, F16, E4M3 = 0, 1, 2, 3
 
 _c_i = ctypes.c_int
 _c_i64 = ctypes.c_int64
@@ -104,6 +104,17 @@ SIGNATURES = {
     "itts_gpt_decode_steps_pl": (_c_i, [_vp, _vp, _vp, _vp, _vp, _c_i, _vp]),
     "itts_bigvgan_workspace_bytes": (_c_i64, [_vp, _c_i, _c_i]),
     "itts_bigvgan_forward": (_c_i, [_vp, _vp, _vp, _vp, _c_i, _c_i, _vp, _vp, _vp, _vp]),
+    "itts_fp8_quant_rows": (_c_i, [_vp, _c_i64, _c_i, _c_i64, _c_i, _vp, _c_i64, _vp, _c_i64, _vp]),
+    "itts_fp8_linear_workspace_bytes": (_c_i64, [_c_i64, _c_i, _c_i]),
+    "itts_fp8_linear": (_c_i, [_vp, _c_i64, _c_i, _c_i64, _c_i, _vp, _c_i64, _vp, _c_i64, _c_i, _vp, _c_i, _vp, _c_i64,
+                               _vp, _c_i64, _c_i, _vp, _vp]),
+    "itts_kv8_write": (_c_i, [_vp, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i, _vp, _vp, _c_i, _vp]),
+    "itts_kv8_read": (_c_i, [_vp, _vp, _vp, _c_i, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i, _vp]),
+    "itts_attn_cached_workspace_bytes": (_c_i64, [_vp, _c_i, _c_i, _c_i, _c_i, _c_i]),
+    "itts_attn_decode_kv8": (_c_i, [_vp, _vp, _c_i64, _c_i64, _c_i, _c_i, _c_i, _vp, _vp, _vp, _c_i64, _c_f, _c_i, _vp,
+                                    _c_i64, _c_i64, _c_i, _vp, _vp]),
+    "itts_attn_tree": (_c_i, [_vp, _vp, _c_i64, _c_i64, _c_i64, _c_i, _c_i, _c_i, _c_i, _vp, _vp, _vp, _vp, _c_i64, _vp,
+                              _c_i64, _c_f, _c_i, _vp, _c_i64, _c_i64, _c_i64, _c_i, _vp, _vp]),
     "itts_diag_occupy": (_c_i, [_c_i, _c_i, _vp, _vp]),
 }
 
@@ -148,6 +159,12 @@ class GptSeqWeights(ctypes.Structure):
 class Sampling(ctypes.Structure):
     _fields_ = [("mode", _c_i), ("min_new", _c_i), ("rep_penalty", _c_f), ("temperature", _c_f), ("top_k", _c_i),
                 ("top_p", _c_f)]
+
+class KvCache(ctypes.Structure):
+    _fields_ = [(n, _vp) for n in ("k", "v", "k_scale", "v_scale")] + \
+        [(n, _c_i64) for n in ("bs", "hs", "sbs", "shs")] + \
+        [(n, _c_i) for n in ("rows", "heads", "max_kv", "head_dim", "dtype")]
+
 
 _lib = None
 _lock = threading.Lock()

@@ -1,0 +1,213 @@
+"""The 8-bit KV cache and the attention over a cache (csrc/kv8.hip, csrc/attn_cached.hip).
+
+``Kv8Cache`` holds one layer's K and V as e4m3 codes [rows, heads, max_kv, head_dim] with one power-of-two scale byte
+per (row, head, position) for each of K and V: (head_dim + 1) / (2 head_dim) of the bf16 cache's bytes.  ``write``
+quantises new tokens into their slots, ``read`` gives slots back, ``decode`` is the single-token attention (left
+padding, the beams' lineage table, shared K/V heads) and ``tree`` the attention of up to 64 drafted tokens per row.
+``Kv16Cache`` is the bf16 decode cache (``[rows, heads, max_kv, head_dim]``, one layer of ``HipGPT``'s) with ``tree``.
+
+Every call runs on the current stream of the cache's device, which must be the current device; nothing synchronises,
+and every argument that changes from step to step lives on the device, so calls may be captured in a graph.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from .. import _hip
+
+_CODE = {torch.float32: _hip.F32, torch.bfloat16: _hip.BF16}
+
+
+class _Cache:
+    """What both caches share: the C view of the tensors, argument checks, the tree attention."""
+
+    def _bind(self, k, v, k_scale, v_scale, dtype):
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride():
+            raise ValueError(f"k and v must be [rows, heads, max_kv, head_dim] alike, got {tuple(k.shape)} and {tuple(v.shape)}")
+        rows, heads, max_kv, hd = k.shape
+        if hd not in (64, 128):
+            raise ValueError(f"head_dim must be 64 or 128, got {hd}")
+        if min(rows, heads, max_kv) < 1:
+            raise ValueError("an empty cache")
+        want = torch.uint8 if dtype == _hip.E4M3 else torch.bfloat16
+        if k.dtype != want or v.dtype != want or not k.is_cuda or v.device != k.device:
+            raise ValueError(f"k and v must be {want} on one GPU")
+        if k.stride(3) != 1 or k.stride(2) != hd:
+            raise ValueError("positions must lie one behind another (strides head_dim and 1)")
+        if k_scale is not None:
+            for s in (k_scale, v_scale):
+                if tuple(s.shape) != (rows, heads, max_kv) or s.dtype != torch.uint8 or s.device != k.device or \
+                        s.stride(2) != 1 or s.stride() != k_scale.stride():
+                    raise ValueError(f"scales must be uint8 [{rows}, {heads}, {max_kv}] with unit position stride")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.rows, self.heads, self.max_kv, self.head_dim, self.dev = rows, heads, max_kv, hd, k.device
+        self._c = _hip.KvCache(k.data_ptr(), v.data_ptr(), _hip.ptr(k_scale), _hip.ptr(v_scale), k.stride(0), k.stride(1),
+                               0 if k_scale is None else k_scale.stride(0), 0 if k_scale is None else k_scale.stride(1),
+                               rows, heads, max_kv, hd, dtype)
+        self._ref = ctypes.byref(self._c)
+        self.lib = _hip.load()
+
+    def _stream(self) -> int:
+        if self.dev.index != torch.cuda.current_device():
+            raise ValueError(f"the cache is on {self.dev}, the current device is cuda:{torch.cuda.current_device()}: "
+                             "call under torch.cuda.device(cache.dev)")
+        return torch.cuda.current_stream().cuda_stream
+
+    def _index(self, t: Optional[torch.Tensor], n: int, name: str) -> Optional[int]:
+        if t is None:
+            return None
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.device != self.dev:
+            raise ValueError(f"{name} must be a contiguous int32 tensor of {n} on {self.dev}")
+        return t.data_ptr()
+
+    def _lineage(self, t: Optional[torch.Tensor], B: int) -> Tuple[Optional[int], int]:
+        if t is None:
+            if B > self.rows:
+                raise ValueError(f"{B} rows over a cache of {self.rows}")
+            return None, 0
+        if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != B or t.shape[1] < self.max_kv or t.stride(1) != 1 or \
+                t.device != self.dev:
+            raise ValueError(f"kv_rows must be int32 [{B}, >= {self.max_kv}] with unit column stride on {self.dev}")
+        return t.data_ptr(), max(t.stride(0), self.max_kv)
+
+    def _heads(self, t: torch.Tensor, name: str) -> int:
+        """query heads per K/V head of t [..., heads * group, head_dim]"""
+        if t.dtype not in _CODE or t.shape[-1] != self.head_dim or t.shape[-2] % self.heads or not t.shape[-2] or \
+                t.stride(-1) != 1 or t.device != self.dev:
+            raise ValueError(f"{name} must be f32 or bf16 [..., a multiple of {self.heads} heads, {self.head_dim}] with unit "
+                             f"last stride on {self.dev}, got {tuple(t.shape)} {t.dtype}")
+        return t.shape[-2] // self.heads
+
+    def _workspace(self, B, T, group, max_len, q):
+        n = self.lib.itts_attn_cached_workspace_bytes(self._ref, B, T, group, max_len, _CODE[q.dtype])
+        if n < 0:
+            raise ValueError("sizes the attention does not take (T <= 64, group <= 4096)")
+        return torch.empty(n, dtype=torch.uint8, device=self.dev) if n else None
+
+    def tree(self, q: torch.Tensor, kv_len: torch.Tensor, mask: torch.Tensor, n_tokens: Optional[torch.Tensor] = None,
+             pad: Optional[torch.Tensor] = None, kv_rows: Optional[torch.Tensor] = None, max_len: Optional[int] = None,
+             scale: Optional[float] = None, out: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16):
+        """Attention of drafted tokens: q [B, T, heads * group, head_dim], T <= 64, their K/V already in the cache behind
+        each row's kv_len [B] accepted positions (drafted token j at position kv_len[b] + j).  mask [B, T] int64 (or [T]:
+        one tree for all rows): bit j of mask[b, t] lets token t see drafted token j; every token also sees the row's
+        positions pad[b] .. kv_len[b] - 1.  n_tokens [B]: drafted tokens of each row (all T if None); the outputs of the
+        others stay as they are in ``out`` (zero without one).  ``tree_mask`` makes masks from parents."""
+        if q.dim() != 4:
+            raise ValueError(f"q must be [B, T, heads, head_dim], got {tuple(q.shape)}")
+        group = self._heads(q, "q")
+        B, T = q.shape[:2]
+        if mask.dtype != torch.int64 or mask.shape not in ((B, T), (T,)) or mask.stride(-1) != 1 and T > 1 or \
+                mask.device != self.dev:
+            raise ValueError(f"mask must be int64 [{B}, {T}] or [{T}] with unit last stride on {self.dev}")
+        if out is None:
+            out = torch.zeros(q.shape, dtype=dtype, device=self.dev)
+        elif out.shape != q.shape or out.stride(3) != 1 or out.dtype not in _CODE or out.device != self.dev:
+            raise ValueError(f"out must be f32 or bf16 {tuple(q.shape)} with unit last stride on {self.dev}")
+        rows, ld = self._lineage(kv_rows, B)
+        longest = self.max_kv if max_len is None else int(max_len)
+        st = self._stream()
+        ws = self._workspace(B, T, group, longest, q)
+        rc = self.lib.itts_attn_tree(
+            self._ref, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), _CODE[q.dtype], B, T, group,
+            self._index(kv_len, B, "kv_len"), self._index(pad, B, "pad"), self._index(n_tokens, B, "n_tokens"),
+            mask.data_ptr(), mask.stride(0) if mask.dim() == 2 else 0, rows, ld,
+            self.head_dim ** -0.5 if scale is None else float(scale), longest, out.data_ptr(), out.stride(0), out.stride(1),
+            out.stride(2), _CODE[out.dtype], _hip.ptr(ws), st)
+        if rc:
+            _hip.check(rc, "itts_attn_tree")
+        return out
+
+
+class Kv16Cache(_Cache):
+    """A bf16 cache [rows, heads, max_kv, head_dim] (one layer of ``HipGPT``'s K and V); the tensors are held, not copied."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor):
+        self._bind(k, v, None, None, _hip.BF16)
+
+
+class Kv8Cache(_Cache):
+    """An e4m3 cache; the tensors are held, not copied (``empty`` makes them)."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        self._bind(k, v, k_scale, v_scale, _hip.E4M3)
+
+    @classmethod
+    def empty(cls, rows: int, heads: int, max_kv: int, head_dim: int = 64, device="cuda:0") -> "Kv8Cache":
+        codes = [torch.zeros(rows, heads, max_kv, head_dim, dtype=torch.uint8, device=device) for _ in range(2)]
+        scales = [torch.zeros(rows, heads, max_kv, dtype=torch.uint8, device=device) for _ in range(2)]
+        return cls(*codes, *scales)
+
+    def write(self, k: torch.Tensor, v: torch.Tensor, row: torch.Tensor, pos: torch.Tensor) -> None:
+        """Quantise k / v [M, heads, head_dim] (f32 or bf16, views of the c_attn output as they are) into the slots
+        (row[i], pos[i]), int32 [M].  A slot outside the cache is skipped (-1 for a padding token); the slots of one
+        call must differ from each other."""
+        for name, t in (("k", k), ("v", v)):
+            if t.dim() != 3 or self._heads(t, name) != 1 or t.dtype != k.dtype or t.shape != k.shape:
+                raise ValueError(f"{name} must be [M, {self.heads}, {self.head_dim}], k and v alike")
+        M = k.shape[0]
+        rc = self.lib.itts_kv8_write(self._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+                                     v.stride(1), _CODE[k.dtype], self._index(row, M, "row"), self._index(pos, M, "pos"), M,
+                                     self._stream())
+        if rc:
+            _hip.check(rc, "itts_kv8_write")
+
+    def read(self, row: torch.Tensor, pos: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
+        """(k, v) [M, heads, head_dim] of the slots (row[i], pos[i]); zeros for a slot outside the cache.  Writing what
+        was read gives the same codes' values again, so an accepted path of drafted tokens moves without loss."""
+        if dtype not in _CODE or row.dim() != 1:
+            raise ValueError("dtype must be f32 or bf16, row [M]")
+        M, hd = row.shape[0], self.head_dim
+        k = torch.empty(M, self.heads, hd, dtype=dtype, device=self.dev)
+        v = torch.empty(M, self.heads, hd, dtype=dtype, device=self.dev)
+        rc = self.lib.itts_kv8_read(self._ref, self._index(row, M, "row"), self._index(pos, M, "pos"), M, k.data_ptr(),
+                                    self.heads * hd, hd, v.data_ptr(), self.heads * hd, hd, _CODE[dtype], self._stream())
+        if rc:
+            _hip.check(rc, "itts_kv8_read")
+        return k, v
+
+    def decode(self, q: torch.Tensor, kv_len: torch.Tensor, pad: Optional[torch.Tensor] = None,
+               kv_rows: Optional[torch.Tensor] = None, max_len: Optional[int] = None, scale: Optional[float] = None,
+               out: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """Single-token attention: q [B, heads * group, head_dim] over positions pad[b] .. kv_len[b] - 1 of each row
+        (this step's K/V written before); scale defaults to head_dim ** -0.5; out bf16 or f32 like q.  kv_rows
+        [B, >= max_kv] int32: the cache row that holds each position (beams).  max_len: the largest kv_len expected
+        (the split over keys is sized by it; default max_kv)."""
+        if q.dim() != 3:
+            raise ValueError(f"q must be [B, heads, head_dim], got {tuple(q.shape)}")
+        group = self._heads(q, "q")
+        B = q.shape[0]
+        if out is None:
+            out = torch.empty(q.shape, dtype=dtype, device=self.dev)
+        elif out.shape != q.shape or out.stride(2) != 1 or out.device != self.dev:
+            raise ValueError(f"out must be {tuple(q.shape)} with unit last stride on {self.dev}")
+        if out.dtype not in _CODE:
+            raise ValueError("out must be f32 or bf16")
+        rows, ld = self._lineage(kv_rows, B)
+        longest = self.max_kv if max_len is None else int(max_len)
+        st = self._stream()
+        ws = self._workspace(B, 1, group, longest, q)
+        rc = self.lib.itts_attn_decode_kv8(
+            self._ref, q.data_ptr(), q.stride(0), q.stride(1), _CODE[q.dtype], B, group,
+            self._index(kv_len, B, "kv_len"), self._index(pad, B, "pad"), rows, ld,
+            self.head_dim ** -0.5 if scale is None else float(scale), longest, out.data_ptr(), out.stride(0), out.stride(1),
+            _CODE[out.dtype], _hip.ptr(ws), st)
+        if rc:
+            _hip.check(rc, "itts_attn_decode_kv8")
+        return out
+
+
+def tree_mask(parents: torch.Tensor) -> torch.Tensor:
+    """Masks int64 [..., T] of trees given by each token's parent [..., T] (an earlier token, or -1 for the last
+    accepted one): bit j of token t is set where j is t or an ancestor of t."""
+    T = parents.shape[-1]
+    if T > 64 or parents.dtype not in (torch.int32, torch.int64):
+        raise ValueError("at most 64 drafted tokens, parents int32 or int64")
+    own = [(1 << t) - (1 << 64 if t == 63 else 0) for t in range(T)]
+    mask = torch.zeros(*parents.shape[:-1], T + 1, dtype=torch.int64, device=parents.device)  # the last: no parent
+    for t in range(T):
+        up = torch.where((parents[..., t] >= 0) & (parents[..., t] < t), parents[..., t], T).long()
+        mask[..., t] = mask.gather(-1, up[..., None])[..., 0] | own[t]
+    return mask[..., :T].contiguous()
