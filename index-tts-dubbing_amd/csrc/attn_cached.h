@@ -17,8 +17,6 @@
 // bf16 output's 2^-9) or, for f32 outputs, as two f16 parts (2^-23).  bf16 V: P as two bf16 parts (2^-17).
 // Maxima, sums and both products accumulate in f32.
 #pragma once
-#include <type_traits>
-
 #include "fp8.h"
 
 namespace itts {
@@ -88,14 +86,22 @@ __device__ __forceinline__ int max_rows(int v) {
 
 constexpr int kWaves = 4;  // waves of a workgroup take its tiles in turn
 
+// waves per SIMD that the registers are held to: the most that leave the loop without spills
+template <bool E4M3, bool LINEAGE, int HD, int QN, int NQ>
+constexpr int waves_per_simd() {
+  if (E4M3 && HD == 64) return NQ == 1 ? 3 : NQ == 2 ? (QN == 1 && !LINEAGE ? 3 : 2) : (QN == 1 ? 2 : 1);
+  if (E4M3 || HD == 64) return NQ == 1 || (NQ == 2 && QN == 1 && !LINEAGE) ? 2 : 1;
+  return 1;
+}
+
 template <bool E4M3, bool LINEAGE, int HD, int QN, int PN, int NQ>
-__global__ __launch_bounds__(64 * kWaves) void attn_cached_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN, NQ>())) void attn_cached_kernel(AttnArgs a) {
   constexpr int ES = E4M3 ? 1 : 2;
   constexpr int KW = HD * ES / 64;  // 16-B pieces of K per lane and 16 keys; dwords of V per lane and key
   constexpr int KS = HD / 32;       // MFMA steps of the first product
   constexpr int DT = HD / 16;       // 16-dim tiles of the second
   constexpr int COLS = 16 * NQ;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, c = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, c = lane >> 4;
   // workgroup -> (unit = (row, K/V head), query block, split).  The query blocks of one (unit, split) read the same keys:
   // they get ids 8 apart, so they land on one XCD one after the other and share its L2
   const int per = 8 * a.qblocks;
@@ -293,7 +299,8 @@ __global__ __launch_bounds__(64 * kWaves) void attn_cached_kernel(AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[j][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  int vref = 0;  // e4m3: V is held relative to 2^(vref - 127)
+  int vref = 0;      // e4m3: V is held relative to 2^(vref - 127)
+  uint32_t odd = 0;  // non-zero: V held a NaN or infinity at a drafted token
 
   // V^T operands [16-dim tile][8 keys]; dim tile d holds the lane's dims (hd / 16) r + d
   auto v_frags = [&](const uint32_t (&v)[8][KW], const float (&sc)[8], u32x4_t (&vf)[DT]) {
@@ -326,9 +333,19 @@ __global__ __launch_bounds__(64 * kWaves) void attn_cached_kernel(AttnArgs a) {
   constexpr uint32_t kOne = E4M3 ? 0x3C00u : 0x3F80u;
   const u32x4_t ones = u32x4_t{kOne * 0x10001u, kOne * 0x10001u, kOne * 0x10001u, kOne * 0x10001u};
 
+  // Which of a tile's 32 keys are seen, as bits: all columns' prefix, and a column's drafted tokens
+  auto below = [](int i) -> uint32_t { return i <= 0 ? 0u : i >= 32 ? ~0u : (1u << i) - 1; };  // bits 0 .. i - 1
+  auto prefix_bits = [&](int tile) { return below(len - tile) & ~below(first - tile); };
+  auto drafted_bits = [&](int tile, uint64_t mask) -> uint32_t {
+    const int d = tile - len;
+    return d >= 64 ? 0u : d >= 0 ? (uint32_t)(mask >> d) : d > -32 ? (uint32_t)(mask << -d) : 0u;
+  };
+  auto mine = [&](uint32_t bits) { return (bits >> (4 * c) & 0xFu) | (bits >> (16 + 4 * c) & 0xFu) << 4; };
+
   // A drafted token's V that is not finite reaches only the columns that see it.  Such values enter the products as 0;
   // here a product of (1 where V is the special value) and (1 where the column sees the key) counts them.
   auto not_finite = [&](int tile) {
+    const uint32_t drafted = mine(below(hi - tile) & ~below(len - tile));
     uint32_t w8[8][KW];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
@@ -347,10 +364,9 @@ __global__ __launch_bounds__(64 * kWaves) void attn_cached_kernel(AttnArgs a) {
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         one[u] = 1.f;
-        const int p = key(tile, u);
 #pragma unroll
         for (int i = 0; i < KW; ++i) {
-          const uint32_t w = p >= len && p < hi ? w8[u][i] : 0u;
+          const uint32_t w = drafted >> u & 1 ? w8[u][i] : 0u;
           uint32_t v = 0;
           if constexpr (E4M3) {
             v = ((((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7) * 0x38u;  // e4m3 1.0
@@ -370,16 +386,10 @@ __global__ __launch_bounds__(64 * kWaves) void attn_cached_kernel(AttnArgs a) {
       const float what = kind == 0 ? __builtin_nanf("") : kind == 1 ? __builtin_inff() : -__builtin_inff();
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
+        const uint32_t vis = mine(drafted_bits(tile, msk[j]));
         u32x4_t pf;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          pf[e] = 0;
-#pragma unroll
-          for (int s2 = 0; s2 < 2; ++s2) {
-            const int p = key(tile, 2 * e + s2);
-            if (p >= len && p < hi && (msk[j] >> ((p - len) & 63) & 1)) pf[e] |= kOne << (16 * s2);
-          }
-        }
+        for (int e = 0; e < 4; ++e) pf[e] = (vis >> (2 * e) & 1) * kOne | (vis >> (2 * e + 1) & 1) * (kOne << 16);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           const f32x4_t count = pv(nf[d], pf, f32x4_t{0.f, 0.f, 0.f, 0.f});
@@ -391,25 +401,23 @@ __global__ __launch_bounds__(64 * kWaves) void attn_cached_kernel(AttnArgs a) {
     }
   };
 
-  // EDGE: the tile holds keys that some column may not see (before the padding's end, drafted, behind the row's end)
-  auto process = [&](const int tile, auto edge_tag) {
-    constexpr bool EDGE = decltype(edge_tag)::value;
+  for (; base < end; base += 32 * kWaves) {
+    const int tile = base;
+    // an edge tile holds keys that some column may not see (before the padding's end, drafted, behind the row's end)
+    const bool edge = tile < first || tile + 32 > len;
     uint32_t some = 0xFF;  // which of the lane's eight keys some column may see
-    uint32_t odd = 0;      // non-zero: V holds a NaN or infinity at a drafted token
-    if constexpr (EDGE) {
-      some = 0;
+    if (edge) {
+      const uint32_t drafted = mine(below(hi - tile) & ~below(len - tile));
+      some = mine(prefix_bits(tile)) | drafted;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const int p = key(tile, u);
-        if (p < len ? p >= first : p < hi) some |= 1u << u;
 #pragma unroll
         for (int i = 0; i < KW; ++i) {
           const uint32_t w = some >> u & 1 ? tv[u][i] : 0u;
           uint32_t bits;  // a drafted token's values that are not finite
           if constexpr (E4M3) bits = (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
           else bits = (((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u) >> 15;
-          if (p < len) bits = 0;
-          bits *= E4M3 ? 0xFFu : 0xFFFFu;
+          bits *= (drafted >> u & 1) * (E4M3 ? 0xFFu : 0xFFFFu);
           odd |= bits;
           tv[u][i] = w & ~bits;
         }
@@ -422,7 +430,10 @@ __global__ __launch_bounds__(64 * kWaves) void attn_cached_kernel(AttnArgs a) {
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         vs[u] = tvs[u >> 2] >> (8 * (u & 3)) & 0xFF;
-        if (EDGE && !(some >> u & 1)) vs[u] = 0;  // nothing is seen of it: no part in the reference, V is 0
+      }
+      if (edge) {  // what nothing is seen of has no part in the reference; its V is 0
+#pragma unroll
+        for (int u = 0; u < 8; ++u) vs[u] = some >> u & 1 ? vs[u] : 0;
       }
       int top = max(max(max(vs[0], vs[1]), max(vs[2], vs[3])), max(max(vs[4], vs[5]), max(vs[6], vs[7])));
       top = __builtin_amdgcn_readfirstlane(max_rows(top));  // 16 lanes each hold the same eight bytes
@@ -477,26 +488,18 @@ __global__ __launch_bounds__(64 * kWaves) void attn_cached_kernel(AttnArgs a) {
       uint32_t vis = 0xFF;
 #pragma unroll
       for (int u = 0; u < 8; ++u) x[u] = s[u >> 2][u & 3];
-      if constexpr (EDGE) {
-        vis = 0;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int p = key(tile, u);
-          const bool see = p < len ? p >= first : p < hi && (msk[j] >> ((p - len) & 63) & 1);
-          vis |= (uint32_t)see << u;
-        }
-      }
       if (any_bad) {
 #pragma unroll
         for (int u = 0; u < 8; ++u) x[u] = bad >> u & 1 ? __builtin_nanf("") : x[u];
       }
-      if constexpr (EDGE) {
+      if (edge) {
+        vis = mine(prefix_bits(tile) | drafted_bits(tile, msk[j]));
 #pragma unroll
         for (int u = 0; u < 8; ++u) x[u] = vis >> u & 1 ? x[u] : -__builtin_inff();
       }
       float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-      // a.qk_scale >= 0; a column that sees nothing of this tile has no maximum (0 * -inf is none)
-      top = EDGE && vis == 0 ? -__builtin_inff() : top * a.qk_scale;
+      top = top * a.qk_scale;  // positive
+
       top = max_rows(top);
       if (__any(top > m[j] + kLag) || rescale != 1.f) {
         const float next = fmaxf(m[j], top);
@@ -512,7 +515,7 @@ __global__ __launch_bounds__(64 * kWaves) void attn_cached_kernel(AttnArgs a) {
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const float z = fmaf(x[u], a.qk_scale, shift);
-        p[u] = __builtin_amdgcn_exp2f(EDGE ? (vis >> u & 1 ? z : -__builtin_inff()) : z);
+        p[u] = __builtin_amdgcn_exp2f(z);
       }
 #pragma unroll
       for (int q = 0; q < PN; ++q) {
@@ -534,14 +537,10 @@ __global__ __launch_bounds__(64 * kWaves) void attn_cached_kernel(AttnArgs a) {
         for (int d = 0; d < DT; ++d) o[j][d] = pv(vf[d], pf, o[j][d]);
       }
     }
-    if constexpr (EDGE) {
-      if (__any(odd != 0)) not_finite(tile);
-    }
-  };
-
-  for (; base < end; base += 32 * kWaves) {
-    if (base < first || base + 32 > len) process(base, std::true_type{});
-    else process(base, std::false_type{});
+  }
+  if (__any(odd != 0)) {  // the drafted tokens' tiles of this wave once more
+    for (int tile = begin + 32 * wave; tile < end; tile += 32 * kWaves)
+      if (tile + 32 > len) not_finite(tile);
   }
 
   // ---- the waves' parts: common maximum and V reference, then O and the sums added in wave order ----

@@ -1,5 +1,8 @@
 // The C entries of attention over a cache (kernels: attn_cached.h): argument checks, the split over keys, the join of
 // the splits' parts.
+#include <cfloat>
+#include <cmath>
+
 #include "attn_cached.h"
 
 namespace {
@@ -77,7 +80,7 @@ int attend(const char* fn, AttnArgs& a, int B, int q_dtype, int out_dtype, int m
   const int cols = a.T * a.G, hd = a.c.head_dim;
   const int qs = a.q_f32 ? 4 : 2, os = a.out_f32 ? 4 : 2;
   a.negate = a.qk_scale < 0.f;
-  a.qk_scale = a.negate ? -a.qk_scale : a.qk_scale;
+  a.qk_scale = fmaxf(fabsf(a.qk_scale), FLT_MIN);  // 0: every score is 0 but for what underflows, and -inf stays -inf
   a.q_vec = ((uintptr_t)a.q & 15) == 0 && ((a.q_sb | a.q_st | a.q_sh) * qs) % 16 == 0;
   a.o_vec = ((uintptr_t)a.out & 15) == 0 && ((a.o_sb | a.o_st | a.o_sh) * os) % 16 == 0;
   a.units = B * a.c.heads;
