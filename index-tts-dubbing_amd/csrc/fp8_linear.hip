@@ -7,6 +7,8 @@
 // 13 bits below it (measured on normal data: 1.5e-5 of the result's rms; the bf16 result rounds by 1.7e-3).
 // f32 outputs: codes times scale are exact in bf16, and v_mfma_f32_16x16x32_bf16 adds exact products to f32 (measured
 // 1.2e-8 of the rms), at half the rate and one conversion per two codes.
+#include <type_traits>
+
 #include "fp8.h"
 
 namespace {
@@ -94,10 +96,11 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
 // ---- product ------------------------------------------------------------------------------------
 // gelu_tanh(v) = v / (1 + exp(-2 u)), u = sqrt(2 / pi) (v + 0.044715 v^3); SiLU(v) = v / (1 + exp(-v)): one exp2 and one
 // reciprocal each (both within about an ulp) instead of tanhf's branches, which cost more than the product did
-__device__ __forceinline__ float apply_act(float v, int act) {
-  if (act == 0) return v;
+template <int ACT>
+__device__ __forceinline__ float apply_act(float v) {
+  if constexpr (ACT == 0) return v;
   constexpr float kLog2e = 1.4426950408889634f, kA = -2.f * 0.7978845608028654f * kLog2e;
-  const float e = act == 1 ? v * fmaf(kA * 0.044715f, v * v, kA) : -kLog2e * v;
+  const float e = ACT == 1 ? v * fmaf(kA * 0.044715f, v * v, kA) : -kLog2e * v;
   return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(e));
 }
 
@@ -115,32 +118,143 @@ struct LinearArgs {
   bool out_bf16, vec_out;
 };
 
-// 16 consecutive outputs n .. n + 15 of row m (bias added): activation, residual, store
-__device__ __forceinline__ void store16(const LinearArgs& p, int64_t m, int n, float (&v)[16]) {
-  if (m >= p.M) return;
+// ---- epilogue of the tile kernels ----
+// Activation and residual are compile-time: with a test per value (and the wait for an optional load beside each store) the
+// epilogue of a 256 x 256 tile took 22 us, more than its products over k = 1024.
+template <int WN>
+constexpr int kPitch = WN + 4;  // floats: rows r and r + 1 four banks apart
+template <int WN>
+constexpr int kBand = 16 * kPitch<WN> * 4;  // bytes of a wave's band
+
+// A sum as a vector register.  AGPR: it stays in its accumulator register until here (left to itself the compiler copies a
+// wave's 256 sums at once, and spills).
+template <bool AGPR>
+__device__ __forceinline__ float sum_of(float a) {
+  if constexpr (!AGPR) return a;
+  float v;
+  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(a));
+  return v;
+}
+template <bool AGPR>
+__device__ __forceinline__ f32x4_t sums_of(f32x4_t a) {
+  return f32x4_t{sum_of<AGPR>(a[0]), sum_of<AGPR>(a[1]), sum_of<AGPR>(a[2]), sum_of<AGPR>(a[3])};
+}
+
+// N a multiple of 16 and aligned rows: a lane's 16 neighbouring results from registers, the four lane groups' 64 side by
+// side.  A row's residual is requested before the stores of the row before (a load waits for the stores before it).
+template <bool BF16, bool AGPR, int ACT, bool RES, int FM, int FN>
+__device__ __forceinline__ void store_direct(const LinearArgs& p, f32x4_t (&acc)[FM][FN], int64_t m0, int n0) {
+  constexpr int G = FN / 4;
+  const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
+  const int left = (int)(p.M - m0 < 16 * FM ? p.M - m0 : 16 * FM);  // rows of the wave's tile
+  f32x4_t bias[G][4], res[RES ? G : 1][4];
+  bool in[G];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    v[i] = apply_act(v[i], p.act);
-    if (p.residual) v[i] += p.residual[m * p.ldr + min(n + i, p.N - 1)];
+  for (int g = 0; g < G; ++g) {
+    const int n = n0 + 64 * g + 16 * c;
+    in[g] = n < p.N;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      bias[g][i] = p.bias && in[g] ? *reinterpret_cast<const f32x4_t*>(p.bias + n + 4 * i) : f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  if (p.vec_out && n + 16 <= p.N) {
-    if (p.out_bf16) {
-      u32x4_t* d = reinterpret_cast<u32x4_t*>((uint16_t*)p.y + m * p.ldy + n);
+  auto load_res = [&](int i) {
+    if constexpr (RES) {
+      const int row = 16 * i + r;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        d[h] = u32x4_t{pack2bf(v[8 * h], v[8 * h + 1]), pack2bf(v[8 * h + 2], v[8 * h + 3]),
-                       pack2bf(v[8 * h + 4], v[8 * h + 5]), pack2bf(v[8 * h + 6], v[8 * h + 7])};
-    } else {
-      f32x4_t* d = reinterpret_cast<f32x4_t*>((float*)p.y + m * p.ldy + n);
+      for (int g = 0; g < G; ++g)
+        if (in[g] && row < left) {
+          const float* src = p.residual + (m0 + row) * p.ldr + n0 + 64 * g + 16 * c;
 #pragma unroll
-      for (int h = 0; h < 4; ++h) d[h] = f32x4_t{v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
+          for (int j = 0; j < 4; ++j) res[g][j] = *reinterpret_cast<const f32x4_t*>(src + 4 * j);
+        }
     }
+  };
+  load_res(0);
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    __builtin_amdgcn_sched_barrier(0);  // row by row: the sums leave the accumulator registers as they are needed
+    const int row = 16 * i + r;
+    f32x4_t v[G][4];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[g][j][e] = apply_act<ACT>(sum_of<AGPR>(acc[i][4 * g + j][e]) + bias[g][j][e]);
+        if constexpr (RES) v[g][j] = v[g][j] + res[g][j];
+      }
+    if (i + 1 < FM) load_res(i + 1);
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      if (in[g] && row < left) {
+        const int64_t at = (m0 + row) * p.ldy + n0 + 64 * g + 16 * c;
+        if constexpr (BF16) {
+          u32x4_t* d = reinterpret_cast<u32x4_t*>((uint16_t*)p.y + at);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            d[h] = u32x4_t{pack2bf(v[g][2 * h][0], v[g][2 * h][1]), pack2bf(v[g][2 * h][2], v[g][2 * h][3]),
+                           pack2bf(v[g][2 * h + 1][0], v[g][2 * h + 1][1]), pack2bf(v[g][2 * h + 1][2], v[g][2 * h + 1][3])};
+        } else {
+          f32x4_t* d = reinterpret_cast<f32x4_t*>((float*)p.y + at);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) d[j] = v[g][j];
+        }
+      }
+  }
+}
+
+// Any N and pitch: bands of 16 rows go through the wave's own part of the LDS, then lanes walk the rows with neighbouring
+// columns, so that whole lines are written all the same (57 us instead of 101 at 1337 x 1000 x 8194).
+template <bool BF16, bool AGPR, int ACT, bool RES, int FM, int FN>
+__device__ __forceinline__ void store_banded(const LinearArgs& p, f32x4_t (&acc)[FM][FN], float* band, int64_t m0, int n0) {
+  constexpr int WN = 16 * FN, CI = WN / 64;
+  const int lane = threadIdx.x & 63, fr = lane & 15, fc = lane >> 4;
+  const int left = (int)(p.M - m0 < 16 * FM ? p.M - m0 : 16 * FM);
+  float bias[CI];
+#pragma unroll
+  for (int k = 0; k < CI; ++k) bias[k] = p.bias ? p.bias[min(n0 + lane + 64 * k, p.N - 1)] : 0.f;
+#pragma unroll
+  for (int b = 0; b < FM; ++b) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+      *reinterpret_cast<f32x4_t*>(&band[fr * kPitch<WN> + 64 * (j >> 2) + 16 * fc + 4 * (j & 3)]) = sums_of<AGPR>(acc[b][j]);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the band is this wave's own: no barrier
+#pragma unroll 1
+    for (int t = 0; t < min(16, left - 16 * b); t += 4) {  // four rows a turn; the band's last rows may be none of M's
+      float v[4][CI];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int k = 0; k < CI; ++k) {
+          v[u][k] = apply_act<ACT>(band[(t + u) * kPitch<WN> + lane + 64 * k] + bias[k]);
+          if constexpr (RES) {
+            const int row = min(16 * b + t + u, left - 1), col = min(n0 + lane + 64 * k, p.N - 1);
+            v[u][k] += p.residual[(m0 + row) * p.ldr + col];
+          }
+        }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int k = 0; k < CI; ++k) {
+          const int row = 16 * b + t + u, col = n0 + lane + 64 * k;
+          if (row < left && col < p.N) {
+            if constexpr (BF16) ((uint16_t*)p.y)[(m0 + row) * p.ldy + col] = f2bf(v[u][k]);
+            else ((float*)p.y)[(m0 + row) * p.ldy + col] = v[u][k];
+          }
+        }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+}
+template <bool BF16, bool AGPR, int ACT, int FM, int FN>
+__device__ __forceinline__ void store_tile(const LinearArgs& p, f32x4_t (&acc)[FM][FN], float* band, int64_t m0, int n0) {
+  if (m0 >= p.M) return;
+  if (p.vec_out) {
+    if (p.residual) store_direct<BF16, AGPR, ACT, true>(p, acc, m0, n0);
+    else store_direct<BF16, AGPR, ACT, false>(p, acc, m0, n0);
   } else {
-    for (int i = 0; i < 16; ++i) {
-      if (n + i >= p.N) break;
-      if (p.out_bf16) ((uint16_t*)p.y)[m * p.ldy + n + i] = f2bf(v[i]);
-      else ((float*)p.y)[m * p.ldy + n + i] = v[i];
-    }
+    if (p.residual) store_banded<BF16, AGPR, ACT, true>(p, acc, band, m0, n0);
+    else store_banded<BF16, AGPR, ACT, false>(p, acc, band, m0, n0);
   }
 }
 
@@ -169,7 +283,9 @@ __device__ __forceinline__ bf16x8_t dequant8(int lo, int hi, float scale) {
 // the four lane groups' 64: whole lines are written without going through LDS.
 typedef __attribute__((address_space(3))) void lds_void;
 
-template <bool EXACT, int BM, int BN, int WM, int WN>
+constexpr int kScaleBlocks = 64;  // blocks of k whose scales the LDS holds at once
+
+template <bool EXACT, int ACT, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void fp8_linear_tile_kernel(LinearArgs p) {
   constexpr int NWN = BN / WN, NW = (BM / WM) * NWN;
   constexpr int FM = WM / 16, FN = WN / 16;
@@ -177,6 +293,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void fp8_linear_tile_ke
   static_assert(WN % 64 == 0 && XI * 8 * NW == BM && WI * 8 * NW == BN, "whole instructions, whole groups of 64 columns");
   // separate arrays: the compiler then sees that reads of one step do not wait for the DMA into the other
   __shared__ __attribute__((aligned(1024))) uint8_t sx0[BM * 128], sx1[BM * 128], sw0[BN * 128], sw1[BN * 128];
+  __shared__ __attribute__((aligned(16))) uint8_t ss[(BM + BN) * kScaleBlocks];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, c = lane >> 4;
   const int wm = (wave / NWN) * WM, wn = (wave % NWN) * WN;
@@ -213,24 +330,35 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void fp8_linear_tile_ke
       __builtin_amdgcn_global_load_lds(static_cast<const void*>(wbase + (int64_t)kb * 128 + woff[i]),
                                        (lds_void*)(W + 1024 * (wave * WI + i)), 16, 0, 0);
   };
-  // scale bytes of the lane's rows, four blocks to a dword
-  const uint8_t *xsr[FM], *wsr[FN];
-#pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int64_t m = m0 + wm + 16 * i + r;
-    xsr[i] = p.xs + (m < p.M ? m : p.M - 1) * p.ldxs;
-  }
-#pragma unroll
-  for (int j = 0; j < FN; ++j) {
-    const int n = n0 + wn + 64 * (j >> 2) + 16 * (r >> 2) + 4 * (j & 3) + (r & 3);
-    wsr[j] = p.ws + (int64_t)min(n, p.N - 1) * p.ldws;
-  }
+  // The scale bytes of kScaleBlocks blocks, x's rows then w's in the order of the LDS rows; dword d of row i at
+  // d ^ (i / 4) % 16, so that a fragment's 16 rows lie on distinct banks.  (Fetched from memory as they are needed, 16 rows
+  // far apart at a time, they cost as much as the products.)
+  auto stage_scales = [&](int kb) {
+    for (int row = threadIdx.x; row < BM + BN; row += 64 * NW) {
+      const uint8_t* src;
+      if (row < BM) {
+        const int64_t left = p.M - 1 - m0;
+        src = p.xs + (m0 + (row < left ? row : left)) * p.ldxs;
+      } else {
+        const int i = row - BM, n = (i & ~63) + 16 * (i >> 2 & 3) + 4 * (i >> 4 & 3) + (i & 3);
+        src = p.ws + (int64_t)min(n0 + n, p.N - 1) * p.ldws;
+      }
+      for (int d = 0; d < min(kScaleBlocks, p.KB - kb + 3) >> 2; ++d)
+        ((uint32_t*)ss)[row * (kScaleBlocks / 4) + (d ^ (row >> 2 & 15))] = ((const uint32_t*)(src + kb))[d];
+    }
+  };
   uint32_t xsc[FM], wsc[FN];
-  auto scales = [&](int kb) {
+  auto scales = [&](int kb) {  // four blocks' bytes of the lane's rows
 #pragma unroll
-    for (int i = 0; i < FM; ++i) xsc[i] = *reinterpret_cast<const uint32_t*>(xsr[i] + kb);
+    for (int i = 0; i < FM; ++i) {
+      const int row = wm + 16 * i + r;
+      xsc[i] = ((const uint32_t*)ss)[row * (kScaleBlocks / 4) + ((kb >> 2 & 15) ^ (row >> 2 & 15))];
+    }
 #pragma unroll
-    for (int j = 0; j < FN; ++j) wsc[j] = *reinterpret_cast<const uint32_t*>(wsr[j] + kb);
+    for (int j = 0; j < FN; ++j) {
+      const int row = BM + wn + 16 * j + r;
+      wsc[j] = ((const uint32_t*)ss)[row * (kScaleBlocks / 4) + ((kb >> 2 & 15) ^ (row >> 2 & 15))];
+    }
   };
 
   f32x4_t acc[FM][FN];
@@ -283,39 +411,220 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void fp8_linear_tile_ke
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+    if ((kb & (kScaleBlocks - 1)) == 0 && kb) {  // everyone has read the scales before
+      stage_scales(kb);
+      __syncthreads();
+    }
     if (kb + 1 < p.KB) issue(kb + 1, nextX, nextW);
-    compute(X, W);
-    if (((kb + 1) & 3) == 0 && kb + 1 < p.KB) {
-      scales(kb + 1);
+    if ((kb & 3) == 0) {
+      scales(kb);
     } else {
 #pragma unroll
       for (int i = 0; i < FM; ++i) xsc[i] >>= 8;
 #pragma unroll
       for (int j = 0; j < FN; ++j) wsc[j] >>= 8;
     }
+    compute(X, W);
   };
   issue(0, sx0, sw0);
-  scales(0);
+  stage_scales(0);
   for (int kb = 0; kb < p.KB; kb += 2) {
     step(kb, sx0, sw0, sx1, sw1);
     if (kb + 1 < p.KB) step(kb + 1, sx1, sw1, sx0, sw0);
   }
+  __syncthreads();  // the steps' LDS becomes the waves' bands
+  static_assert((NW + 3) / 4 * kBand<WN> <= (BM < BN ? BM : BN) * 128, "the bands fit");
+  uint8_t* const part = (wave & 2) ? (wave & 1 ? sw1 : sw0) : (wave & 1 ? sx1 : sx0);
+  store_tile<!EXACT, false, ACT>(p, acc, (float*)(part + (wave >> 2) * kBand<WN>), m0 + wm, n0 + wn);
+}
+
+// ---- large tiles ----
+// 256 x 256 outputs in four waves of 128 x 128, one per SIMD: a wave's 16 fragments feed 64 products, so a step costs the
+// LDS 1536 clocks (128 KB read, 64 KB written by the DMA, 128 B a clock) against the matrix unit's 2048; with waves of
+// 128 x 64 both take 2048.  One wave per SIMD has to overlap by itself, so a step is straight-line code in rows of eight
+// products with the fragments of later rows requested between them.  The step's one barrier stands before its last three
+// rows, when all of the step's fragments are in registers: behind it the step's LDS is free for the DMA of the step after
+// next, which has a whole step to land, and the next step's fragments are read under the last rows' products.
+// Rows of x behind M are read from the workspace's padding (their results are not stored); rows of w behind N by the
+// bounds of the buffer resource as 0.
+template <typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const T* p, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, (uint32_t)(bytes < 0xFFFFFFFFll ? bytes : 0xFFFFFFFFll), 0x00020000);
+}
+
+// The 256 accumulator registers of a wave are all sums.  As a builtin the compiler moves a third of them on every turn of the
+// loop and spills; as assembly they stay.  A sum is next touched 64 products later, operands come from the LDS (the
+// compiler waits for those), and what the vector unit writes or reads next to a product is kept apart by s_nop.
+template <int S>  // which byte of the scale registers
+__device__ __forceinline__ void product_agpr(f32x4_t& acc, const i32x8_t& w, const i32x8_t& x, uint32_t ws, uint32_t xs) {
+  if constexpr (S == 0)
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]"
+                 : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs));
+  else
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0]"
+                 : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs));
+}
+// the matrix unit has finished and the vector unit's writes have landed, for every sum
+template <int F>
+__device__ __forceinline__ void settle(f32x4_t (&acc)[F][F]) {
 #pragma unroll
-  for (int g = 0; g < FN / 4; ++g) {
-    const int n = n0 + wn + 64 * g + 16 * c;
-    float bias[16];
+  for (int i = 0; i < F; ++i)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) bias[i] = p.bias ? p.bias[min(n + i, p.N - 1)] : 0.f;
+    for (int j = 0; j < F; ++j) asm volatile("" : "+a"(acc[i][j]));
+  asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      float v[16];
+  for (int i = 0; i < F; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < F; ++j) asm volatile("" : "+a"(acc[i][j]));
+}
+
+template <int ACT>
+__global__ __launch_bounds__(256, 1) void fp8_linear_large_kernel(LinearArgs p) {
+  constexpr int F = 8;
+  __shared__ __attribute__((aligned(1024))) uint8_t sx0[256 * 128], sx1[256 * 128], sw0[256 * 128], sw1[256 * 128];
+  __shared__ __attribute__((aligned(16))) uint8_t ss[512 * kScaleBlocks];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, c = lane >> 4;
+  const int wm = (wave >> 1) * 128, wn = (wave & 1) * 128;
+  const int ntn = (p.N + 255) / 256;
+  const int nblk = gridDim.x, q8 = nblk / 8, r8 = nblk % 8;
+  const int xcd = blockIdx.x % 8, lid = xcd * q8 + min(xcd, r8) + blockIdx.x / 8;
+  const int64_t m0 = (int64_t)(lid / ntn) * 256;
+  const int n0 = (lid % ntn) * 256;
+
+  // DMA instruction i of a wave fills LDS rows 64 wave + 8 i + dr; its lanes' rows and swizzle depend on i's parity alone
+  const int dr = lane >> 3, ds = lane & 7;
+  const int ldx = (int)p.ldxq, ldw = (int)p.ldw;
+  const auto xrs = buffer_of(p.xq + m0 * ldx, (int64_t)256 * ldx);
+  const auto wrs = buffer_of(p.wq + (int64_t)n0 * ldw, (int64_t)(p.N - n0) * ldw);
+  uint32_t xoff[2], woff[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * j + e] = acc[i][4 * g + j][e] + bias[4 * j + e];
-      store16(p, m0 + wm + 16 * i + r, n, v);
+  for (int i = 0; i < 2; ++i) {
+    const int chunk = 16 * (ds ^ (4 * i + (dr >> 1)));
+    xoff[i] = dr * ldx + chunk;
+    woff[i] = (16 * (dr >> 2) + (dr & 3)) * ldw + chunk;
+  }
+  // x's and w's rows of a step: eight instructions each
+  auto issue_x = [&](int i, int kb, uint8_t* X) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(xrs, (lds_void*)(X + 1024 * (wave * F + i)), 16, xoff[i & 1],
+                                             (64 * wave + 8 * i) * ldx + 128 * kb, 0, 0);
+  };
+  auto issue_w = [&](int i, int kb, uint8_t* W) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(wrs, (lds_void*)(W + 1024 * (wave * F + i)), 16, woff[i & 1],
+                                             (64 * wave + 32 * (i & 1) + 4 * (i >> 1)) * ldw + 128 * kb, 0, 0);
+  };
+  // All of the tile's scale bytes, x's rows then w's in the order of its LDS rows; dword d of row i at d ^ (i / 4) % 16, so
+  // that a fragment's 16 rows lie on distinct banks.  (Fetched from memory as they are needed, 16 rows far apart at a time,
+  // they cost as much as the products.)
+  {
+    const int row = threadIdx.x, swz = row >> 2 & 15;
+    const int64_t left = p.M - 1 - m0;
+    const uint32_t* xs = (const uint32_t*)(p.xs + (m0 + (row < left ? row : left)) * p.ldxs);
+    const int n = (row & ~63) + 16 * (row >> 2 & 3) + 4 * (row >> 4 & 3) + (row & 3);
+    const uint32_t* ws = (const uint32_t*)(p.ws + (int64_t)min(n0 + n, p.N - 1) * p.ldws);
+    for (int d = 0; d < (p.KB + 3) >> 2; ++d) {
+      ((uint32_t*)ss)[row * (kScaleBlocks / 4) + (d ^ swz)] = xs[d];
+      ((uint32_t*)ss)[(256 + row) * (kScaleBlocks / 4) + (d ^ swz)] = ws[d];
     }
   }
+  uint32_t xsc[F], wsc[F];  // two blocks' bytes of the lane's rows
+  auto scales = [&](int kb, uint32_t (&x)[F], uint32_t (&w)[F]) {
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      // rows wm + 16 i + r and wn + 16 i + r: row / 4 % 16 = (4 i + r / 4) % 16
+      const int at = 4 * ((kb >> 2) ^ ((4 * i + (r >> 2)) & 15)) + (kb & 2);
+      x[i] = *reinterpret_cast<const uint16_t*>(ss + (wm + 16 * i + r) * kScaleBlocks + at);
+      w[i] = *reinterpret_cast<const uint16_t*>(ss + (256 + wn + 16 * i + r) * kScaleBlocks + at);
+    }
+  };
+  f32x4_t acc[F][F];
+#pragma unroll
+  for (int i = 0; i < F; ++i)
+#pragma unroll
+    for (int j = 0; j < F; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const int a0 = r * 128 + ((c ^ (r >> 1 & 7)) << 4), a1 = r * 128 + (((4 + c) ^ (r >> 1 & 7)) << 4);
+  auto read = [&](const uint8_t* s, int row) -> i32x8_t {
+    const u32x4_t lo = *reinterpret_cast<const u32x4_t*>(s + row * 128 + a0), hi = *reinterpret_cast<const u32x4_t*>(s + row * 128 + a1);
+    return i32x8_t{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+  };
+  i32x8_t w[F], xf[4];
+  // one step (S: byte of the scales): W's fragments in w, row 0's in xf[0]; leaves the next step's there
+  auto step = [&](auto tag, int kb, uint8_t* X, uint8_t* W, uint8_t* nextX, uint8_t* nextW) {
+    constexpr int S = decltype(tag)::value;
+    auto product = [&](int i, int j) { product_agpr<S>(acc[i][j], w[j], xf[i & 3], wsc[j], xsc[i]); };
+    const int next = min(kb + 1, p.KB - 1), after = min(kb + 2, p.KB - 1);
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+      if (i == 0) xf[1] = read(X, wm + 16);
+      if (i < 4) xf[(i + 2) & 3] = read(X, wm + 16 * (i + 2));
+      if (i == 4) {
+        xf[2] = read(X, wm + 16 * 6);
+        xf[3] = read(X, wm + 16 * 7);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < F; ++j) {
+        product(i, j);
+        if (i < 2 && (j & 1)) {  // the rest of the next step's DMA, a few products apart: a burst holds up the products
+          issue_w(4 * i + (j >> 1), next, nextW);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);  // this step's fragments are here, this wave's part of the next has landed
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    xf[0] = read(nextX, wm);
+#pragma unroll
+    for (int j = 0; j < F; ++j) {
+      product(5, j);
+      product(6, j);
+      product(7, j);
+      w[j] = read(nextW, wn + 16 * j);
+      issue_x(j, after, X);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < F; ++i) {
+    issue_x(i, 0, sx0);
+    issue_w(i, 0, sw0);
+  }
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  scales(0, xsc, wsc);
+#pragma unroll
+  for (int j = 0; j < F; ++j) w[j] = read(sw0, wn + 16 * j);
+  xf[0] = read(sx0, wm);
+#pragma unroll
+  for (int i = 0; i < F; ++i) issue_x(i, min(1, p.KB - 1), sx1);
+  settle(acc);
+  using std::integral_constant;
+  int kb = 0;
+  for (; kb + 2 <= p.KB; kb += 2) {
+    uint32_t xn[F], wnx[F];
+    scales(min(kb + 2, (p.KB - 1) & ~1), xn, wnx);
+    step(integral_constant<int, 0>{}, kb, sx0, sw0, sx1, sw1);
+    step(integral_constant<int, 1>{}, kb + 1, sx1, sw1, sx0, sw0);
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      xsc[i] = xn[i];
+      wsc[i] = wnx[i];
+    }
+#pragma unroll
+    for (int i = 0; i < F; ++i) asm volatile("" : "+v"(xsc[i]), "+v"(wsc[i]));
+    asm volatile("s_nop 7" ::: "memory");
+  }
+  if (kb < p.KB) step(integral_constant<int, 0>{}, kb, sx0, sw0, sx1, sw1);
+  __builtin_amdgcn_s_waitcnt(0x0070);  // the last steps' DMA repeats the last block into LDS that nothing reads
+  settle(acc);
+  __syncthreads();  // the steps' LDS becomes the waves' bands
+  uint8_t* const part = (wave & 2) ? (wave & 1 ? sw1 : sw0) : (wave & 1 ? sx1 : sx0);
+  store_tile<true, true, ACT>(p, acc, (float*)part, m0 + wm, n0 + wn);
 }
 
 // ---- few rows ----
@@ -402,7 +711,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void fp8_linear_few_kernel(LinearAr
     const int64_t m = m0 + row;
     const int n = n0 + col;
     if (m < p.M && n < p.N) {
-      v = apply_act(v + (p.bias ? p.bias[n] : 0.f), p.act);
+      v += p.bias ? p.bias[n] : 0.f;
+      v = p.act == 0 ? v : p.act == 1 ? apply_act<1>(v) : apply_act<2>(v);
       if (p.residual) v += p.residual[m * p.ldr + n];
       if (p.out_bf16) ((uint16_t*)p.y)[m * p.ldy + n] = f2bf(v);
       else ((float*)p.y)[m * p.ldy + n] = v;
@@ -429,27 +739,30 @@ int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 int64_t code_pitch(int K) { return round_up(K, 128); }
 int64_t scale_pitch(int K) { return round_up(round_up(K, 128) / 128, 4); }
 
-#ifndef FEWM
-#define FEWM 256
-#endif
-bool few_rows(int64_t M, int N) { return M <= FEWM; }
+// Few rows: one launch of the small kernel, whose rate (it quantises x once per 16 columns of y) is some 90 TFLOP/s, against a
+// quantising pass and tiles.  Measured, us (this / 128 x 128 tiles): 96 x 4096 x 1024 17 / 44, 96 x 1024 x 4096 15 / 16,
+// 300 x 1024 x 1024 14 / 15, 2000 x 1024 x 4096 195 / 22.
+bool few_rows(int64_t M, int N, int K) { return M <= 32 || M * N * (int64_t)K <= 500000000; }
+// 256 x 256 tiles once they keep most of the 256 CUs busy (and the scales of all of k fit the LDS beside them).  Measured,
+// us (these / 128 x 128): 14400 x 1024 x 4096 107 / 122, 8192 x 8192 x 8192 467 / 657, 2000 x 1024 x 4096 (128 tiles) 26 / 22.
+bool large_tiles(int64_t M, int N, int K) { return ((M + 255) / 256) * ((N + 255) / 256) >= 200 && K <= 128 * kScaleBlocks; }
 
 template <bool EXACT, int BM, int BN, int WM, int WN>
 void launch_tile(const LinearArgs& p, hipStream_t st) {
-  const int64_t g = ((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
-  hipLaunchKernelGGL((fp8_linear_tile_kernel<EXACT, BM, BN, WM, WN>), dim3((unsigned)g), dim3(64 * (BM / WM) * (BN / WN)), 0, st, p);
+  const dim3 g((unsigned)(((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN))), b(64 * (BM / WM) * (BN / WN));
+  if (p.act == 0) hipLaunchKernelGGL((fp8_linear_tile_kernel<EXACT, 0, BM, BN, WM, WN>), g, b, 0, st, p);
+  else if (p.act == 1) hipLaunchKernelGGL((fp8_linear_tile_kernel<EXACT, 1, BM, BN, WM, WN>), g, b, 0, st, p);
+  else hipLaunchKernelGGL((fp8_linear_tile_kernel<EXACT, 2, BM, BN, WM, WN>), g, b, 0, st, p);
+}
+void launch_large(const LinearArgs& p, hipStream_t st) {
+  const dim3 g((unsigned)(((p.M + 255) / 256) * ((p.N + 255) / 256))), b(256);
+  if (p.act == 0) hipLaunchKernelGGL(fp8_linear_large_kernel<0>, g, b, 0, st, p);
+  else if (p.act == 1) hipLaunchKernelGGL(fp8_linear_large_kernel<1>, g, b, 0, st, p);
+  else hipLaunchKernelGGL(fp8_linear_large_kernel<2>, g, b, 0, st, p);
 }
 #ifndef VAR
 #define VAR 0
 #endif
-template <bool EXACT>
-void launch_tiles(const LinearArgs& p, hipStream_t st) {
-  if (VAR == 0) launch_tile<EXACT, 256, 256, 128, 64>(p, st);
-  else if (VAR == 1) launch_tile<EXACT, 128, 128, 64, 64>(p, st);
-  else if (VAR == 2) launch_tile<EXACT, 128, 256, 64, 64>(p, st);
-  else if (VAR == 3) launch_tile<EXACT, 256, 128, 128, 64>(p, st);
-  else if (VAR == 4) launch_tile<EXACT, 64, 128, 32, 64>(p, st);
-}
 template <typename T>
 void launch_few(const T* x, int64_t ldx, int K, bool vec, const LinearArgs& p, hipStream_t st) {
   const int mt = p.M <= 16 ? 1 : 2;
@@ -479,7 +792,7 @@ extern "C" int itts_fp8_quant_rows(const void* x, int64_t ldx, int x_dtype, int6
 
 extern "C" int64_t itts_fp8_linear_workspace_bytes(int64_t M, int N, int K) {
   if (M < 0 || N < 1 || N > kMaxN || K < 1 || K > kMaxK || M > ((int64_t)1 << 40) / code_pitch(K)) return -1;
-  return round_up(M * (code_pitch(K) + scale_pitch(K)), 256);
+  return round_up(M, 256) * (code_pitch(K) + scale_pitch(K));  // whole tiles of rows
 }
 
 extern "C" int itts_fp8_linear(const void* x, int64_t ldx, int x_dtype, int64_t M, int K, const uint8_t* wq, int64_t ldw,
@@ -491,26 +804,29 @@ extern "C" int itts_fp8_linear(const void* x, int64_t ldx, int x_dtype, int64_t 
   ITTS_REQUIRE(act >= 0 && act <= 2, fn, "act must be 0 (none), 1 (gelu_tanh) or 2 (SiLU)");
   ITTS_REQUIRE(itts_fp8_linear_workspace_bytes(M, N, K) >= 0 && ldx >= K && ldy >= N && (!residual || ldr >= N), fn,
                "bad sizes");
-  ITTS_REQUIRE(ldw >= code_pitch(K) && ldw % 16 == 0 && ldws >= scale_pitch(K) && ldws % 4 == 0, fn,
-               "weight rows need K rounded up to 128 bytes, scale rows ceil(K / 128) rounded up to 4");
+  ITTS_REQUIRE(ldw >= code_pitch(K) && ldw % 16 == 0 && ldws >= scale_pitch(K) && ldws % 4 == 0 && ldw <= 4 * kMaxK &&
+                   ldws <= kMaxK,
+               fn, "weight rows need K rounded up to 128 bytes, scale rows ceil(K / 128) rounded up to 4");
   if (M == 0) return 0;
   ITTS_REQUIRE(x && wq && ws && y && workspace, fn, "null pointer");
   ITTS_REQUIRE((((uintptr_t)wq | (uintptr_t)workspace) & 15) == 0 && ((uintptr_t)ws & 3) == 0, fn, "misaligned pointer");
-  ITTS_REQUIRE((M + 63) / 64 <= 65535, fn, "too many rows for one launch");
+  ITTS_REQUIRE(((M + 127) / 128) * ((N + 127) / 128) <= 0x7FFFFFFF, fn, "too many tiles for one launch");
   uint8_t* xq = (uint8_t*)workspace;
-  uint8_t* xs = xq + M * code_pitch(K);
+  uint8_t* xs = xq + round_up(M, 256) * code_pitch(K);
   hipStream_t st = itts::as_stream(stream);
   const int es = out_dtype == ITTS_F32 ? 4 : 2;
   LinearArgs p{xq, xs, wq, ws, code_pitch(K), scale_pitch(K), ldw, ldws, M, N, (K + 127) / 128, bias, residual, ldr, y, ldy,
-               act, out_dtype == ITTS_BF16, ((uintptr_t)y & 15) == 0 && (ldy * es) % 16 == 0};
-  if (few_rows(M, N)) {
+               act, out_dtype == ITTS_BF16, ((uintptr_t)y & 15) == 0 && (ldy * es) % 16 == 0 && N % 16 == 0 &&
+                   ((uintptr_t)bias & 15) == 0 && ((uintptr_t)residual & 15) == 0 && (!residual || ldr % 4 == 0)};
+  if (few_rows(M, N, K)) {
     const bool vec = ((uintptr_t)x & 15) == 0 && ldx % (x_dtype == ITTS_F32 ? 4 : 8) == 0;
     if (x_dtype == ITTS_F32) launch_few((const float*)x, ldx, K, vec, p, st);
     else launch_few((const uint16_t*)x, ldx, K, vec, p, st);
     return itts::check_launch(fn);
   }
   if (int rc = launch_quant(fn, x, ldx, x_dtype, M, K, xq, code_pitch(K), xs, scale_pitch(K), st)) return rc;
-  if (p.out_bf16) launch_tiles<false>(p, st);
-  else launch_tiles<true>(p, st);
+  if (!p.out_bf16) launch_tile<true, 128, 128, 64, 64>(p, st);
+  else if (large_tiles(M, N, K)) launch_large(p, st);
+  else launch_tile<false, 128, 128, 64, 64>(p, st);
   return itts::check_launch(fn);
 }
