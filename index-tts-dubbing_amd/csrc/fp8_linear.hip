@@ -792,7 +792,7 @@ extern "C" int itts_fp8_quant_rows(const void* x, int64_t ldx, int x_dtype, int6
 
 extern "C" int64_t itts_fp8_linear_workspace_bytes(int64_t M, int N, int K) {
   if (M < 0 || N < 1 || N > kMaxN || K < 1 || K > kMaxK || M > ((int64_t)1 << 40) / code_pitch(K)) return -1;
-  return round_up(M, 256) * (code_pitch(K) + scale_pitch(K));  // whole tiles of rows
+  return few_rows(M, N, K) ? 0 : round_up(M, 256) * (code_pitch(K) + scale_pitch(K));  // whole tiles of rows
 }
 
 extern "C" int itts_fp8_linear(const void* x, int64_t ldx, int x_dtype, int64_t M, int K, const uint8_t* wq, int64_t ldw,
@@ -808,7 +808,8 @@ extern "C" int itts_fp8_linear(const void* x, int64_t ldx, int x_dtype, int64_t 
                    ldws <= kMaxK,
                fn, "weight rows need K rounded up to 128 bytes, scale rows ceil(K / 128) rounded up to 4");
   if (M == 0) return 0;
-  ITTS_REQUIRE(x && wq && ws && y && workspace, fn, "null pointer");
+  const bool few = few_rows(M, N, K);
+  ITTS_REQUIRE(x && wq && ws && y && (few || workspace), fn, "null pointer");
   ITTS_REQUIRE((((uintptr_t)wq | (uintptr_t)workspace) & 15) == 0 && ((uintptr_t)ws & 3) == 0, fn, "misaligned pointer");
   ITTS_REQUIRE(((M + 127) / 128) * ((N + 127) / 128) <= 0x7FFFFFFF, fn, "too many tiles for one launch");
   uint8_t* xq = (uint8_t*)workspace;
@@ -818,7 +819,7 @@ extern "C" int itts_fp8_linear(const void* x, int64_t ldx, int x_dtype, int64_t 
   LinearArgs p{xq, xs, wq, ws, code_pitch(K), scale_pitch(K), ldw, ldws, M, N, (K + 127) / 128, bias, residual, ldr, y, ldy,
                act, out_dtype == ITTS_BF16, ((uintptr_t)y & 15) == 0 && (ldy * es) % 16 == 0 && N % 16 == 0 &&
                    ((uintptr_t)bias & 15) == 0 && ((uintptr_t)residual & 15) == 0 && (!residual || ldr % 4 == 0)};
-  if (few_rows(M, N, K)) {
+  if (few) {
     const bool vec = ((uintptr_t)x & 15) == 0 && ldx % (x_dtype == ITTS_F32 ? 4 : 8) == 0;
     if (x_dtype == ITTS_F32) launch_few((const float*)x, ldx, K, vec, p, st);
     else launch_few((const uint16_t*)x, ldx, K, vec, p, st);

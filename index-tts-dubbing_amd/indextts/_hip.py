@@ -214,6 +214,15 @@ def stream_ptr(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def current_stream_of(index: int) -> int:
+    """Raw current stream of the device ``index``, which must be the current device: a kernel launched on another
+    device's stream would run on the wrong one.  (The raw query: building a Stream object costs more than a launch.)"""
+    if torch._C._cuda_getDevice() != index:
+        raise ValueError(f"the tensors are on cuda:{index}, the current device is cuda:{torch.cuda.current_device()}: "
+                         "call under torch.cuda.device(tensor.device)")
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def dtype_code(t) -> int:
     if t.dtype == torch.float32:
         return F32

@@ -43,23 +43,19 @@ class _Cache:
                         s.stride(2) != 1 or s.stride() != k_scale.stride():
                     raise ValueError(f"scales must be uint8 [{rows}, {heads}, {max_kv}] with unit position stride")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.rows, self.heads, self.max_kv, self.head_dim, self.dev = rows, heads, max_kv, hd, k.device
+        self.rows, self.heads, self.max_kv, self.head_dim = rows, heads, max_kv, hd
+        self.dev, self.index = k.device, k.get_device()
         self._c = _hip.KvCache(k.data_ptr(), v.data_ptr(), _hip.ptr(k_scale), _hip.ptr(v_scale), k.stride(0), k.stride(1),
                                0 if k_scale is None else k_scale.stride(0), 0 if k_scale is None else k_scale.stride(1),
                                rows, heads, max_kv, hd, dtype)
         self._ref = ctypes.byref(self._c)
+        self.scale = hd ** -0.5
         self.lib = _hip.load()
-
-    def _stream(self) -> int:
-        if self.dev.index != torch.cuda.current_device():
-            raise ValueError(f"the cache is on {self.dev}, the current device is cuda:{torch.cuda.current_device()}: "
-                             "call under torch.cuda.device(cache.dev)")
-        return torch.cuda.current_stream().cuda_stream
 
     def _index(self, t: Optional[torch.Tensor], n: int, name: str) -> Optional[int]:
         if t is None:
             return None
-        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.device != self.dev:
+        if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous() or t.get_device() != self.index:
             raise ValueError(f"{name} must be a contiguous int32 tensor of {n} on {self.dev}")
         return t.data_ptr()
 
@@ -69,20 +65,21 @@ class _Cache:
                 raise ValueError(f"{B} rows over a cache of {self.rows}")
             return None, 0
         if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != B or t.shape[1] < self.max_kv or t.stride(1) != 1 or \
-                t.device != self.dev:
+                t.get_device() != self.index:
             raise ValueError(f"kv_rows must be int32 [{B}, >= {self.max_kv}] with unit column stride on {self.dev}")
         return t.data_ptr(), max(t.stride(0), self.max_kv)
 
-    def _heads(self, t: torch.Tensor, name: str) -> int:
+    def _heads(self, t: torch.Tensor, shape, name: str) -> int:
         """query heads per K/V head of t [..., heads * group, head_dim]"""
-        if t.dtype not in _CODE or t.shape[-1] != self.head_dim or t.shape[-2] % self.heads or not t.shape[-2] or \
-                t.stride(-1) != 1 or t.device != self.dev:
+        group = shape[-2] // self.heads
+        if t.dtype not in _CODE or shape[-1] != self.head_dim or not group or shape[-2] != group * self.heads or \
+                t.stride(-1) != 1 or t.get_device() != self.index:
             raise ValueError(f"{name} must be f32 or bf16 [..., a multiple of {self.heads} heads, {self.head_dim}] with unit "
-                             f"last stride on {self.dev}, got {tuple(t.shape)} {t.dtype}")
-        return t.shape[-2] // self.heads
+                             f"last stride on {self.dev}, got {tuple(shape)} {t.dtype}")
+        return group
 
-    def _workspace(self, B, T, group, max_len, q):
-        n = self.lib.itts_attn_cached_workspace_bytes(self._ref, B, T, group, max_len, _CODE[q.dtype])
+    def _workspace(self, B, T, group, max_len, q_dtype):
+        n = self.lib.itts_attn_cached_workspace_bytes(self._ref, B, T, group, max_len, q_dtype)
         if n < 0:
             raise ValueError("sizes the attention does not take (T <= 64, group <= 4096)")
         return torch.empty(n, dtype=torch.uint8, device=self.dev) if n else None
@@ -95,27 +92,31 @@ class _Cache:
         one tree for all rows): bit j of mask[b, t] lets token t see drafted token j; every token also sees the row's
         positions pad[b] .. kv_len[b] - 1.  n_tokens [B]: drafted tokens of each row (all T if None); the outputs of the
         others stay as they are in ``out`` (zero without one).  ``tree_mask`` makes masks from parents."""
-        if q.dim() != 4:
-            raise ValueError(f"q must be [B, T, heads, head_dim], got {tuple(q.shape)}")
-        group = self._heads(q, "q")
-        B, T = q.shape[:2]
-        if mask.dtype != torch.int64 or mask.shape not in ((B, T), (T,)) or mask.stride(-1) != 1 and T > 1 or \
-                mask.device != self.dev:
+        shape = q.shape
+        if len(shape) != 4:
+            raise ValueError(f"q must be [B, T, heads, head_dim], got {tuple(shape)}")
+        group = self._heads(q, shape, "q")
+        B, T = shape[0], shape[1]
+        one = mask.dim() == 1
+        if mask.dtype != torch.int64 or mask.shape != ((T,) if one else (B, T)) or mask.stride(-1) != 1 and T > 1 or \
+                mask.get_device() != self.index:
             raise ValueError(f"mask must be int64 [{B}, {T}] or [{T}] with unit last stride on {self.dev}")
         if out is None:
-            out = torch.zeros(q.shape, dtype=dtype, device=self.dev)
-        elif out.shape != q.shape or out.stride(3) != 1 or out.dtype not in _CODE or out.device != self.dev:
-            raise ValueError(f"out must be f32 or bf16 {tuple(q.shape)} with unit last stride on {self.dev}")
+            out = torch.zeros(shape, dtype=dtype, device=self.dev)
+        elif out.shape != shape or out.stride(3) != 1 or out.get_device() != self.index:
+            raise ValueError(f"out must be {tuple(shape)} with unit last stride on {self.dev}")
+        qd, od = _CODE[q.dtype], _CODE.get(out.dtype)
+        if od is None or od == _hip.F32 and self._c.dtype == _hip.BF16:
+            raise ValueError("out must be bf16, or f32 over an 8-bit cache")
         rows, ld = self._lineage(kv_rows, B)
         longest = self.max_kv if max_len is None else int(max_len)
-        st = self._stream()
-        ws = self._workspace(B, T, group, longest, q)
+        ws = self._workspace(B, T, group, longest, qd)
+        qs, os = q.stride(), out.stride()
         rc = self.lib.itts_attn_tree(
-            self._ref, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), _CODE[q.dtype], B, T, group,
-            self._index(kv_len, B, "kv_len"), self._index(pad, B, "pad"), self._index(n_tokens, B, "n_tokens"),
-            mask.data_ptr(), mask.stride(0) if mask.dim() == 2 else 0, rows, ld,
-            self.head_dim ** -0.5 if scale is None else float(scale), longest, out.data_ptr(), out.stride(0), out.stride(1),
-            out.stride(2), _CODE[out.dtype], _hip.ptr(ws), st)
+            self._ref, q.data_ptr(), qs[0], qs[1], qs[2], qd, B, T, group, self._index(kv_len, B, "kv_len"),
+            self._index(pad, B, "pad"), self._index(n_tokens, B, "n_tokens"), mask.data_ptr(), 0 if one else mask.stride(0),
+            rows, ld, self.scale if scale is None else float(scale), longest, out.data_ptr(), os[0], os[1], os[2], od,
+            None if ws is None else ws.data_ptr(), _hip.current_stream_of(self.index))
         if rc:
             _hip.check(rc, "itts_attn_tree")
         return out
@@ -144,26 +145,28 @@ class Kv8Cache(_Cache):
         """Quantise k / v [M, heads, head_dim] (f32 or bf16, views of the c_attn output as they are) into the slots
         (row[i], pos[i]), int32 [M].  A slot outside the cache is skipped (-1 for a padding token); the slots of one
         call must differ from each other."""
-        for name, t in (("k", k), ("v", v)):
-            if t.dim() != 3 or self._heads(t, name) != 1 or t.dtype != k.dtype or t.shape != k.shape:
-                raise ValueError(f"{name} must be [M, {self.heads}, {self.head_dim}], k and v alike")
-        M = k.shape[0]
-        rc = self.lib.itts_kv8_write(self._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                                     v.stride(1), _CODE[k.dtype], self._index(row, M, "row"), self._index(pos, M, "pos"), M,
-                                     self._stream())
+        shape = k.shape
+        if len(shape) != 3 or v.shape != shape or v.dtype != k.dtype or self._heads(k, shape, "k") != 1 or \
+                self._heads(v, shape, "v") != 1:
+            raise ValueError(f"k and v must be [M, {self.heads}, {self.head_dim}], alike")
+        M, ks, vs = shape[0], k.stride(), v.stride()
+        rc = self.lib.itts_kv8_write(self._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _CODE[k.dtype],
+                                     self._index(row, M, "row"), self._index(pos, M, "pos"), M,
+                                     _hip.current_stream_of(self.index))
         if rc:
             _hip.check(rc, "itts_kv8_write")
 
     def read(self, row: torch.Tensor, pos: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
         """(k, v) [M, heads, head_dim] of the slots (row[i], pos[i]); zeros for a slot outside the cache.  Writing what
         was read gives the same codes' values again, so an accepted path of drafted tokens moves without loss."""
-        if dtype not in _CODE or row.dim() != 1:
+        code = _CODE.get(dtype)
+        if code is None or row.dim() != 1:
             raise ValueError("dtype must be f32 or bf16, row [M]")
-        M, hd = row.shape[0], self.head_dim
-        k = torch.empty(M, self.heads, hd, dtype=dtype, device=self.dev)
-        v = torch.empty(M, self.heads, hd, dtype=dtype, device=self.dev)
-        rc = self.lib.itts_kv8_read(self._ref, self._index(row, M, "row"), self._index(pos, M, "pos"), M, k.data_ptr(),
-                                    self.heads * hd, hd, v.data_ptr(), self.heads * hd, hd, _CODE[dtype], self._stream())
+        M, H, hd = row.shape[0], self.heads, self.head_dim
+        kv = torch.empty((2, M, H, hd), dtype=dtype, device=self.dev)
+        k, v = kv.unbind(0)
+        rc = self.lib.itts_kv8_read(self._ref, self._index(row, M, "row"), self._index(pos, M, "pos"), M, k.data_ptr(), H * hd,
+                                    hd, v.data_ptr(), H * hd, hd, code, _hip.current_stream_of(self.index))
         if rc:
             _hip.check(rc, "itts_kv8_read")
         return k, v
@@ -175,25 +178,26 @@ class Kv8Cache(_Cache):
         (this step's K/V written before); scale defaults to head_dim ** -0.5; out bf16 or f32 like q.  kv_rows
         [B, >= max_kv] int32: the cache row that holds each position (beams).  max_len: the largest kv_len expected
         (the split over keys is sized by it; default max_kv)."""
-        if q.dim() != 3:
-            raise ValueError(f"q must be [B, heads, head_dim], got {tuple(q.shape)}")
-        group = self._heads(q, "q")
-        B = q.shape[0]
+        shape = q.shape
+        if len(shape) != 3:
+            raise ValueError(f"q must be [B, heads, head_dim], got {tuple(shape)}")
+        group = self._heads(q, shape, "q")
+        B = shape[0]
         if out is None:
-            out = torch.empty(q.shape, dtype=dtype, device=self.dev)
-        elif out.shape != q.shape or out.stride(2) != 1 or out.device != self.dev:
-            raise ValueError(f"out must be {tuple(q.shape)} with unit last stride on {self.dev}")
-        if out.dtype not in _CODE:
+            out = torch.empty(shape, dtype=dtype, device=self.dev)
+        elif out.shape != shape or out.stride(2) != 1 or out.get_device() != self.index:
+            raise ValueError(f"out must be {tuple(shape)} with unit last stride on {self.dev}")
+        qd, od = _CODE[q.dtype], _CODE.get(out.dtype)
+        if od is None:
             raise ValueError("out must be f32 or bf16")
         rows, ld = self._lineage(kv_rows, B)
         longest = self.max_kv if max_len is None else int(max_len)
-        st = self._stream()
-        ws = self._workspace(B, 1, group, longest, q)
+        ws = self._workspace(B, 1, group, longest, qd)
+        qs, os = q.stride(), out.stride()
         rc = self.lib.itts_attn_decode_kv8(
-            self._ref, q.data_ptr(), q.stride(0), q.stride(1), _CODE[q.dtype], B, group,
-            self._index(kv_len, B, "kv_len"), self._index(pad, B, "pad"), rows, ld,
-            self.head_dim ** -0.5 if scale is None else float(scale), longest, out.data_ptr(), out.stride(0), out.stride(1),
-            _CODE[out.dtype], _hip.ptr(ws), st)
+            self._ref, q.data_ptr(), qs[0], qs[1], qd, B, group, self._index(kv_len, B, "kv_len"), self._index(pad, B, "pad"),
+            rows, ld, self.scale if scale is None else float(scale), longest, out.data_ptr(), os[0], os[1], od,
+            None if ws is None else ws.data_ptr(), _hip.current_stream_of(self.index))
         if rc:
             _hip.check(rc, "itts_attn_decode_kv8")
         return out

@@ -17,14 +17,6 @@ BLOCK = 128
 _CODE = {torch.float32: _hip.F32, torch.bfloat16: _hip.BF16}
 
 
-def _stream(t: torch.Tensor) -> int:
-    """The current stream of the tensor's device, which must be the current one (a kernel runs there)."""
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}: "
-                         "call under torch.cuda.device(tensor.device)")
-    return torch.cuda.current_stream().cuda_stream
-
-
 def quant_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """x [M, K] f32 or bf16 on the GPU (unit column stride) -> (codes [M, K rounded up to 128] uint8, scale bytes
     [M, K / 128 rounded up to whole dwords] uint8); view the codes as ``torch.float8_e4m3fn`` for their values."""
@@ -41,7 +33,7 @@ def quant_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     q = torch.empty(M, kp, dtype=torch.uint8, device=x.device)
     s = torch.empty(M, sp, dtype=torch.uint8, device=x.device)
     _hip.check(lib.itts_fp8_quant_rows(x.data_ptr(), max(x.stride(0), K), _CODE[x.dtype], M, K, q.data_ptr(), kp,
-                                       s.data_ptr(), sp, _stream(x)), "itts_fp8_quant_rows")
+                                       s.data_ptr(), sp, _hip.current_stream_of(x.get_device())), "itts_fp8_quant_rows")
     return q, s
 
 
@@ -67,9 +59,9 @@ class Fp8Linear:
                                  or bias.device != codes.device):
             raise ValueError(f"bias must be [{N}] f32, contiguous, on {codes.device}")
         self.codes, self.scales, self.bias = codes, scales, bias
-        self.in_features, self.out_features, self.dev = K, N, codes.device
+        self.in_features, self.out_features, self.dev, self.index = K, N, codes.device, codes.get_device()
         self.lib = _hip.load()
-        self._w = (codes.data_ptr(), kp, scales.data_ptr(), sp, N, _hip.ptr(bias))
+        self._w = (codes.data_ptr(), kp, scales.data_ptr(), sp, _hip.ptr(bias))
 
     @classmethod
     def from_weight(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> "Fp8Linear":
@@ -81,35 +73,39 @@ class Fp8Linear:
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """act(x @ W^T + b) (+ residual); act 0 none, 1 gelu_tanh, 2 SiLU; y f32, or bf16 with ``bf16_out``;
         residual f32 [..., N], contiguous, may be ``out`` itself."""
-        K, N = self.in_features, self.out_features
-        if x.dtype not in _CODE or x.dim() < 1 or x.shape[-1] != K or x.device != self.dev:
-            raise ValueError(f"x must be [..., {K}] f32 or bf16 on {self.dev}, got {tuple(x.shape)} {x.dtype} on {x.device}")
-        lead = x.shape[:-1]
-        if x.dim() != 2:
+        K, N, dev = self.in_features, self.out_features, self.index
+        shape = x.shape
+        xd = _CODE.get(x.dtype)
+        if xd is None or not shape or shape[-1] != K or x.get_device() != dev:
+            raise ValueError(f"x must be [..., {K}] f32 or bf16 on {self.dev}, got {tuple(shape)} {x.dtype} on {x.device}")
+        ys = (*shape[:-1], N)
+        if len(shape) != 2:
             x = x.reshape(-1, K)
         M = x.shape[0]
         ldx = x.stride(0) if M > 1 else K
         if K > 1 and x.stride(1) != 1 or ldx < K:
             x = x.contiguous()
             ldx = K
-        dt = torch.bfloat16 if bf16_out else torch.float32
+        dt, yd = (torch.bfloat16, _hip.BF16) if bf16_out else (torch.float32, _hip.F32)
         if out is None:
-            y = torch.empty(*lead, N, dtype=dt, device=self.dev)
+            y = torch.empty(ys, dtype=dt, device=self.dev)
         else:
             y = out
-            if y.dtype != dt or y.shape != (*lead, N) or not y.is_contiguous() or y.device != self.dev:
-                raise ValueError(f"out must be a contiguous {dt} tensor of {(*lead, N)} on {self.dev}")
-        if residual is not None and (residual.dtype != torch.float32 or residual.shape != (*lead, N)
-                                     or not residual.is_contiguous() or residual.device != self.dev):
-            raise ValueError(f"residual must be a contiguous f32 tensor of {(*lead, N)} on {self.dev}")
+            if y.dtype != dt or y.shape != ys or not y.is_contiguous() or y.get_device() != dev:
+                raise ValueError(f"out must be a contiguous {dt} tensor of {ys} on {self.dev}")
+        res = None
+        if residual is not None:
+            if residual.dtype != torch.float32 or residual.shape != ys or not residual.is_contiguous() or \
+                    residual.get_device() != dev:
+                raise ValueError(f"residual must be a contiguous f32 tensor of {ys} on {self.dev}")
+            res = residual.data_ptr()
         if M == 0:
             return y
-        wsb = self.lib.itts_fp8_linear_workspace_bytes(M, N, K)
-        ws = torch.empty(wsb, dtype=torch.uint8, device=self.dev) if wsb > 0 else None
-        wq, ldw, wsc, lds, _, b = self._w
-        rc = self.lib.itts_fp8_linear(x.data_ptr(), ldx, _CODE[x.dtype], M, K, wq, ldw, wsc, lds, N, b, act,
-                                      None if residual is None else residual.data_ptr(), N, y.data_ptr(), N, _CODE[dt],
-                                      None if ws is None else ws.data_ptr(), _stream(x))
+        n = self.lib.itts_fp8_linear_workspace_bytes(M, N, K)
+        ws = torch.empty(n, dtype=torch.uint8, device=self.dev) if n > 0 else None
+        wq, ldw, wsc, lds, b = self._w
+        rc = self.lib.itts_fp8_linear(x.data_ptr(), ldx, xd, M, K, wq, ldw, wsc, lds, N, b, act, res, N, y.data_ptr(), N, yd,
+                                      None if ws is None else ws.data_ptr(), _hip.current_stream_of(dev))
         if rc:
             _hip.check(rc, "itts_fp8_linear")
         return y

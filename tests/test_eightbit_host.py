@@ -91,12 +91,13 @@ def test_linear_calls_refuse(lib):
 
     for kw in (dict(x=None), dict(ldx=199), dict(xd=2), dict(M=-1), dict(K=0), dict(N=0), dict(w=8), dict(ldw=128),
                dict(ldw=260), dict(ws=None), dict(lds=3), dict(act=3), dict(act=-1), dict(res=16, ldr=7), dict(y=None),
-               dict(ldy=7), dict(od=2), dict(wk=None), dict(wk=8), dict(M=1 << 40)):
+               dict(ldy=7), dict(od=2), dict(wk=8), dict(M=1 << 40), dict(M=4096, N=4096, ldy=4096, wk=None)):
         assert linear(**kw) != 0, kw
         assert b"itts_fp8_linear" in lib.itts_last_error()
     assert linear(M=0, x=None, y=None, wk=None) == 0
     assert lib.itts_fp8_linear_workspace_bytes(-1, 8, 8) == -1
-    assert lib.itts_fp8_linear_workspace_bytes(3, 8, 200) >= 3 * (256 + 4)
+    assert lib.itts_fp8_linear_workspace_bytes(3, 8, 200) == 0
+    assert lib.itts_fp8_linear_workspace_bytes(5000, 4096, 200) >= 5000 * (256 + 4)
 
 
 def test_python_refusals_without_gpu():
