@@ -18,26 +18,43 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   const int unit = (int)(id / C), cg = (int)(id - (int64_t)unit * C);
   if (unit >= a.units) return;
   const int b = unit / a.c.heads, h = unit - b * a.c.heads;
+  // lane = (quarter or half of the splits, 4 dims); the first splits' parts are requested before anything else is known
+  constexpr int L = HD / 4, P = 64 / L, EARLY = 4;
+  const int d = 4 * (lane % L), g = lane / L;
+  const int64_t base = (int64_t)unit * a.nsplit * C + cg;
+  auto at = [&](int s) { return base + (int64_t)s * C; };
+  f32x4_t early[EARLY];
+  float em[EARLY], el[EARLY];
+#pragma unroll
+  for (int i = 0; i < EARLY; ++i) {
+    const int64_t e = at(min(g + P * i, a.nsplit - 1));
+    early[i] = *reinterpret_cast<const f32x4_t*>(a.part + e * HD + d);
+    em[i] = a.part_ml[2 * e];
+    el[i] = a.part_ml[2 * e + 1];
+  }
   const int t = cg / a.G;
   const int len = a.kv_len[b];
   const int n = a.tree ? (a.n_tokens ? a.n_tokens[b] : a.T) : 0;
   const bool refuse = len < 0 || n < 0 || n > a.T || len > a.c.max_kv - n;
   if (!refuse && t >= (a.tree ? n : 1)) return;
-  // lane = (quarter or half of the splits, 4 dims)
-  constexpr int L = HD / 4, P = 64 / L;
-  const int d = 4 * (lane % L), g = lane / L;
   float top = -__builtin_inff();
-  for (int s = lane; s < a.nsplit; s += 64) top = fmaxf(top, a.part_ml[2 * (((int64_t)unit * a.nsplit + s) * C + cg)]);
+  for (int s = lane; s < a.nsplit; s += 64) top = fmaxf(top, a.part_ml[2 * at(s)]);
   top = wave_max(top);
   const float ref = top == -__builtin_inff() ? 0.f : top;
   float sum = 0.f;
   f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = g; s < a.nsplit; s += P) {
-    const int64_t at = ((int64_t)unit * a.nsplit + s) * C + cg;
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - ref);
-    sum += f * a.part_ml[2 * at + 1];
-    acc = acc + *reinterpret_cast<const f32x4_t*>(a.part + at * HD + d) * f;
+#pragma unroll
+  for (int i = 0; i < EARLY; ++i) {
+    if (g + P * i < a.nsplit) {
+      const float f = __builtin_amdgcn_exp2f(em[i] - ref);
+      sum += f * el[i];
+      acc = acc + early[i] * f;
+    }
+  }
+  for (int s = g + P * EARLY; s < a.nsplit; s += P) {
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at(s)] - ref);
+    sum += f * a.part_ml[2 * at(s) + 1];
+    acc = acc + *reinterpret_cast<const f32x4_t*>(a.part + at(s) * HD + d) * f;
   }
 #pragma unroll
   for (int o = L; o < 64; o <<= 1) {

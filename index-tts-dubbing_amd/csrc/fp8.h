@@ -32,4 +32,36 @@ __device__ __forceinline__ float e4m3_prescale(float v, float inv) {
   return finite_f(v) ? v * inv : __builtin_nanf("");
 }
 
+// The magnitudes' maximum is taken on their bits: as integers they order like the values, and what is not finite comes out
+// above every finite value, so one test per block finds it and the ordinary path tests no value.  max_bits: of f32 values
+// or of pairs of bf16 (dwords), the result in f32's bits.
+constexpr uint32_t kInfBits = 0x7F800000u;
+__device__ __forceinline__ uint32_t max_bits(const float (&v)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  return m;
+}
+
+// scale byte of N values' block and the values divided by the scale, given the block's largest magnitude's bits
+// (`top`); `reduce`: a value's maximum over the block's lanes.  Values that are not finite become NaN.
+template <int N, typename R>
+__device__ __forceinline__ int e4m3_scaled(float (&v)[N], uint32_t top, R reduce) {
+  if (__any(top >= kInfBits)) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t b = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+      m = max(m, b < kInfBits ? b : 0u);
+      v[i] = b < kInfBits ? v[i] : __builtin_nanf("");
+    }
+    top = reduce(m);
+  }
+  const int byte = e4m3_scale_byte(__uint_as_float(top));
+  const float inv = e4m3_inv_scale(byte);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] *= inv;
+  return byte;
+}
+
 }  // namespace itts

@@ -13,13 +13,10 @@
 
 namespace {
 
-using itts::e4m3_inv_scale;
 using itts::e4m3_pack4;
-using itts::e4m3_prescale;
-using itts::e4m3_scale_byte;
-using itts::finite_f;
 
 typedef __attribute__((ext_vector_type(8))) int i32x8_t;
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
 
 constexpr int kMaxK = 1 << 20;
 constexpr int kMaxN = 1 << 24;
@@ -59,19 +56,15 @@ __device__ __forceinline__ void load_vals<uint16_t>(const uint16_t* row, int k, 
 }
 
 // codes of this lane's 8 values and the scale byte of its 16-lane block
-__device__ __forceinline__ int quant8(const float (&v)[8], u32x2_t& codes) {
-  float a = 0.f;
+__device__ __forceinline__ int quant8(float (&v)[8], u32x2_t& codes) {
+  auto reduce = [](uint32_t m) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a = fmaxf(a, finite_f(v[i]) ? fabsf(v[i]) : 0.f);
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
-  const int byte = e4m3_scale_byte(a);
-  const float inv = e4m3_inv_scale(byte);
-  float q[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) q[i] = e4m3_prescale(v[i], inv);
-  codes[0] = e4m3_pack4(q[0], q[1], q[2], q[3]);
-  codes[1] = e4m3_pack4(q[4], q[5], q[6], q[7]);
+    for (int o = 8; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+    return m;
+  };
+  const int byte = itts::e4m3_scaled(v, reduce(itts::max_bits(v)), reduce);
+  codes[0] = e4m3_pack4(v[0], v[1], v[2], v[3]);
+  codes[1] = e4m3_pack4(v[4], v[5], v[6], v[7]);
   return byte;
 }
 
@@ -633,16 +626,56 @@ __global__ __launch_bounds__(256, 1) void fp8_linear_large_kernel(LinearArgs p) 
 // and no workspace; w's fragments come straight from global memory: with few rows the bytes of w are the cost.
 constexpr int kFewWaves = 8;
 
+// 32 values of a row as they come from memory: chunks k .. +15 and k + 64 .. +79
 template <typename T>
-__device__ __forceinline__ void load16(const T* row, int k, int K, bool vec, float (&v)[16]) {
-  float h[8];
+struct Raw32 {
+  static constexpr int N = sizeof(T);  // 16-B pieces of 16 values: 2 (bf16) or 4 (f32)
+  u32x4_t w[2][N];
+  __device__ __forceinline__ void load(const T* row, int k, int K, bool vec) {
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    load_vals(row, k + 8 * g, K, vec, h);
+    for (int g = 0; g < 2; ++g) {
+      const int kk = k + 64 * g;
+      if (vec && kk + 16 <= K) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[8 * g + i] = h[i];
+        for (int i = 0; i < N; ++i) w[g][i] = *reinterpret_cast<const u32x4_t*>(row + kk + i * (16 / N));
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int at = kk + (16 / N) * i + (4 / N) * e;
+            if constexpr (N == 4) w[g][i][e] = at < K ? __float_as_uint(row[at]) : 0u;
+            else w[g][i][e] = (at < K ? (uint32_t)row[at] : 0u) | (at + 1 < K ? (uint32_t)row[at + 1] << 16 : 0u);
+          }
+      }
+    }
   }
-}
+  __device__ __forceinline__ uint32_t max_bits() const {  // f32 bits of the largest magnitude
+    if constexpr (N == 4) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) m = max(m, w[g][i][e] & 0x7FFFFFFFu);
+      return m;
+    } else {  // two at a time
+      u16x2_t m = {0, 0};
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, w[g][i][e] & 0x7FFF7FFFu));
+      return (uint32_t)max(m[0], m[1]) << 16;
+    }
+  }
+  __device__ __forceinline__ float value(int g, int i) const {  // i: 0 .. 15
+    if constexpr (N == 4) return __uint_as_float(w[g][i >> 2][i & 3]);
+    else return __uint_as_float(i & 1 ? w[g][i >> 3][(i & 7) >> 1] & 0xFFFF0000u : w[g][i >> 3][(i & 7) >> 1] << 16);
+  }
+};
 
 template <bool EXACT, typename T, int MT>
 __global__ __launch_bounds__(64 * kFewWaves) void fp8_linear_few_kernel(LinearArgs p, const T* __restrict__ x, int64_t ldx, int K, bool vec) {
@@ -661,32 +694,39 @@ __global__ __launch_bounds__(64 * kFewWaves) void fp8_linear_few_kernel(LinearAr
   f32x4_t acc[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  // the next block's operands are requested before this one's are used
+  i32x8_t wn;
+  int sn;
+  Raw32<T> xn[MT];
+  auto fetch = [&](int kb) {
+    wn = frag(wr + kb * 128);
+    sn = wsr[kb];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) xn[t].load(xr[t], 128 * kb + 16 * c, K, vec);
+  };
+  if (wave < p.KB) fetch(wave);
   for (int kb = wave; kb < p.KB; kb += kFewWaves) {
-    const i32x8_t wf = frag(wr + kb * 128);
-    const int sw = wsr[kb];
-    float v[MT][2][16];
+    const i32x8_t wf = wn;
+    const int sw = sn;
+    Raw32<T> xc[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int g = 0; g < 2; ++g) load16(xr[t], 128 * kb + 64 * g + 16 * c, K, vec, v[t][g]);
+    for (int t = 0; t < MT; ++t) xc[t] = xn[t];
+    if (kb + kFewWaves < p.KB) fetch(kb + kFewWaves);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      float a = 0.f;
+      float v[32];
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) a = fmaxf(a, finite_f(v[t][g][i]) ? fabsf(v[t][g][i]) : 0.f);
-      a = fmaxf(a, __shfl_xor(a, 16, 64));
-      a = fmaxf(a, __shfl_xor(a, 32, 64));
-      const int sx = e4m3_scale_byte(a);
-      const float inv = e4m3_inv_scale(sx);
+        for (int i = 0; i < 16; ++i) v[16 * g + i] = xc[t].value(g, i);
+      auto reduce = [](uint32_t m) {  // the four lanes of the row
+        m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+        return max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+      };
+      const int sx = itts::e4m3_scaled(v, reduce(xc[t].max_bits()), reduce);
       i32x8_t xf;
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          xf[4 * g + i] = (int)e4m3_pack4(e4m3_prescale(v[t][g][4 * i], inv), e4m3_prescale(v[t][g][4 * i + 1], inv),
-                                          e4m3_prescale(v[t][g][4 * i + 2], inv), e4m3_prescale(v[t][g][4 * i + 3], inv));
+      for (int i = 0; i < 8; ++i) xf[i] = (int)e4m3_pack4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
       if constexpr (EXACT) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)

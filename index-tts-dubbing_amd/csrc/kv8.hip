@@ -3,24 +3,21 @@
 // scale bytes [row][head][pos].
 //
 // Pure traffic: a token and head reads hd values and writes hd + 1 bytes for each of K and V.  hd / 8 lanes per vector,
-// eight values per lane, so a lane's 16-B (bf16) or 32-B (f32) load becomes one 8-B store.
+// eight values per lane, so a lane's 16-B (bf16) or 32-B (f32) load becomes one 8-B store.  What it needs is loads in
+// flight: KVNOTE
 #include "fp8.h"
 
 namespace {
 
-using itts::e4m3_inv_scale;
 using itts::e4m3_pack4;
-using itts::e4m3_prescale;
 using itts::e4m3_scale;
-using itts::e4m3_scale_byte;
-using itts::finite_f;
 
 struct Kv8Args {
   ItTsKvCache c;
   const void *k, *v;  // write: sources; read: destinations
   int64_t k_st, k_sh, v_st, v_sh;
   const int32_t *row, *pos;
-  int64_t units;  // tokens * heads * 2
+  int M, heads, lanes, per_block;  // tokens; heads of a group, their lanes (heads x 2 x hd / 8); tokens side by side
   bool vec;
 };
 
@@ -63,57 +60,78 @@ __device__ __forceinline__ void st8(T* p, bool vec, const float (&v)[8]) {
   }
 }
 
-// unit u = (token * heads + head) * 2 + (0: K, 1: V); lanes 0 .. HD / 8 - 1 of the unit hold 8 values each
-template <typename T, int HD, bool WRITE>
+// The heads are dealt to the eight XCDs (workgroup id % 8), so that a line of the cache -- 128 / hd positions of a head,
+// or 128 positions' scale bytes -- is written or read through one L2 whatever the order of the slots: tokens in random
+// order otherwise cost a partial line in several L2s for each byte.  A token takes (heads of the group) x 2 x HD / 8 lanes
+// (K or V, then head, then eight values), whole workgroups of 256 along grid y where that is more; a lane keeps its place
+// and goes through TURNS tokens whose loads are all in flight together.
+template <typename T, int HD, bool WRITE, int TURNS>
 __global__ __launch_bounds__(256) void kv8_kernel(Kv8Args a) {
   constexpr int L = HD / 8;
-  const int64_t u = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;
-  const int l = threadIdx.x % L;
-  if (u >= a.units) return;  // whole groups of L lanes leave together
-  const bool isv = u & 1;
-  const int64_t th = u >> 1;
-  const int64_t t = th / a.c.heads;
-  const int h = (int)(th - t * a.c.heads);
-  const int row = a.row[t], pos = a.pos[t];
-  const bool ok = (unsigned)row < (unsigned)a.c.rows && (unsigned)pos < (unsigned)a.c.max_kv;
-  const int64_t slot = (int64_t)row * a.c.bs + (int64_t)h * a.c.hs + (int64_t)pos * HD + 8 * l;
-  const int64_t sslot = (int64_t)row * a.c.sbs + (int64_t)h * a.c.shs + pos;
-  uint8_t* codes = (uint8_t*)(isv ? a.c.v : a.c.k);
-  uint8_t* scale = isv ? a.c.v_scale : a.c.k_scale;
-  const int64_t off = t * (isv ? a.v_st : a.k_st) + h * (isv ? a.v_sh : a.k_sh) + 8 * l;
-  float v[8];
+  const int slot = a.per_block > 1 ? (int)threadIdx.x / a.lanes : 0;
+  const int u = blockIdx.y * 256 + threadIdx.x - slot * a.lanes;
+  if (u >= a.lanes || slot >= a.per_block) return;  // whole groups of L lanes leave together
+  const int l = u % L, h = (int)(blockIdx.x & 7) * a.heads + ((u / L) >> 1);
+  if (h >= a.c.heads) return;
+  const bool isv = (u / L) & 1;
+  uint8_t* codes = (uint8_t*)(isv ? a.c.v : a.c.k) + (int64_t)h * a.c.hs + 8 * l;
+  uint8_t* scale = (isv ? a.c.v_scale : a.c.k_scale) + (int64_t)h * a.c.shs;
+  T* side = (T*)const_cast<void*>(isv ? a.v : a.k) + h * (isv ? a.v_sh : a.k_sh) + 8 * l;
+  const int64_t st = isv ? a.v_st : a.k_st;
+  const int64_t t0 = ((int64_t)(blockIdx.x >> 3) * a.per_block + slot) * TURNS;
+  if (t0 >= a.M) return;
+  bool ok[TURNS];
+  int64_t cs[TURNS], ss[TURNS];
+#pragma unroll
+  for (int i = 0; i < TURNS; ++i) {
+    const int64_t t = t0 + i < a.M ? t0 + i : a.M - 1;
+    const int row = a.row[t], pos = a.pos[t];
+    ok[i] = (unsigned)row < (unsigned)a.c.rows && (unsigned)pos < (unsigned)a.c.max_kv;
+    cs[i] = ok[i] ? (int64_t)row * a.c.bs + (int64_t)pos * HD : 0;
+    ss[i] = ok[i] ? (int64_t)row * a.c.sbs + pos : 0;
+  }
   if constexpr (WRITE) {
-    if (!ok) return;
-    ld8((const T*)(isv ? a.v : a.k) + off, a.vec, v);
-    float m = 0.f;
+    float v[TURNS][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_f(v[i]) ? fabsf(v[i]) : 0.f);
+    for (int i = 0; i < TURNS; ++i) ld8(side + (t0 + i < a.M ? t0 + i : a.M - 1) * st, a.vec, v[i]);
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    const int byte = e4m3_scale_byte(m);
-    const float inv = e4m3_inv_scale(byte);
-    float q[8];
+    for (int i = 0; i < TURNS; ++i) {
+      auto reduce = [](uint32_t m) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = e4m3_prescale(v[i], inv);
-    *reinterpret_cast<u32x2_t*>(codes + slot) =
-        u32x2_t{e4m3_pack4(q[0], q[1], q[2], q[3]), e4m3_pack4(q[4], q[5], q[6], q[7])};
-    if (l == 0) scale[sslot] = (uint8_t)byte;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    if (ok) {
-      const u32x2_t c = *reinterpret_cast<const u32x2_t*>(codes + slot);
-      const float s = e4m3_scale(scale[sslot]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(c[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(c[i], true);
-        v[4 * i] = lo[0] * s;
-        v[4 * i + 1] = lo[1] * s;
-        v[4 * i + 2] = hi[0] * s;
-        v[4 * i + 3] = hi[1] * s;
+        for (int o = L / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+        return m;
+      };
+      const int byte = itts::e4m3_scaled(v[i], reduce(itts::max_bits(v[i])), reduce);
+      const float(&q)[8] = v[i];
+      if (ok[i] && t0 + i < a.M) {
+        *reinterpret_cast<u32x2_t*>(codes + cs[i]) =
+            u32x2_t{e4m3_pack4(q[0], q[1], q[2], q[3]), e4m3_pack4(q[4], q[5], q[6], q[7])};
+        if (l == 0) scale[ss[i]] = (uint8_t)byte;
       }
     }
-    st8((T*)(isv ? const_cast<void*>(a.v) : const_cast<void*>(a.k)) + off, a.vec, v);
+  } else {
+    u32x2_t c[TURNS];
+    int byte[TURNS];
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) {
+      c[i] = *reinterpret_cast<const u32x2_t*>(codes + cs[i]);
+      byte[i] = scale[ss[i]];
+    }
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) {
+      if (t0 + i >= a.M) break;
+      const float s = e4m3_scale(byte[i]);
+      float v[8];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(c[i][g], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(c[i][g], true);
+        v[4 * g] = ok[i] ? lo[0] * s : 0.f;
+        v[4 * g + 1] = ok[i] ? lo[1] * s : 0.f;
+        v[4 * g + 2] = ok[i] ? hi[0] * s : 0.f;
+        v[4 * g + 3] = ok[i] ? hi[1] * s : 0.f;
+      }
+      st8(side + (t0 + i) * st, a.vec, v);
+    }
   }
 }
 
@@ -128,17 +146,26 @@ int launch(const char* fn, const ItTsKvCache* c, const void* k, int64_t k_st, in
   ITTS_REQUIRE(k && v && row && pos, fn, "null pointer");
   const int es = dtype == ITTS_F32 ? 4 : 2;
   const bool vec = (((uintptr_t)k | (uintptr_t)v) & 15) == 0 && ((k_st | k_sh | v_st | v_sh) * es) % 16 == 0;
-  Kv8Args a{*c, k, v, k_st, k_sh, v_st, v_sh, row, pos, (int64_t)M * c->heads * 2, vec};
-  const int64_t blocks = (a.units * (c->head_dim / 8) + 255) / 256;
-  ITTS_REQUIRE(blocks <= 0x7FFFFFFF, fn, "too many tokens for one launch");
+  // four tokens a lane where that leaves workgroups enough, one where latency counts
+  const int turns = M >= 4096 ? 4 : 1;
+  const int group = (c->heads + 7) / 8;
+  const int64_t lanes = (int64_t)group * 2 * (c->head_dim / 8);
+  const int per = lanes < 256 ? (int)(256 / lanes) : 1;
+  Kv8Args a{*c, k, v, k_st, k_sh, v_st, v_sh, row, pos, M, group, (int)lanes, per, vec};
+  const int64_t blocks = 8 * ((M + (int64_t)per * turns - 1) / ((int64_t)per * turns)), deep = (lanes + 255) / 256;
+  ITTS_REQUIRE(deep <= 65535 && blocks <= 0x7FFFFFFF, fn, "too many tokens or heads for one launch");
   hipStream_t s = itts::as_stream(stream);
-  const dim3 g((unsigned)blocks), b(256);
+  const dim3 g((unsigned)blocks, (unsigned)deep), b(256);
+  auto go = [&](auto kernel4, auto kernel1) {
+    if (turns == 4) hipLaunchKernelGGL(kernel4, g, b, 0, s, a);
+    else hipLaunchKernelGGL(kernel1, g, b, 0, s, a);
+  };
   if (dtype == ITTS_F32) {
-    if (c->head_dim == 64) hipLaunchKernelGGL((kv8_kernel<float, 64, WRITE>), g, b, 0, s, a);
-    else hipLaunchKernelGGL((kv8_kernel<float, 128, WRITE>), g, b, 0, s, a);
+    if (c->head_dim == 64) go(kv8_kernel<float, 64, WRITE, 4>, kv8_kernel<float, 64, WRITE, 1>);
+    else go(kv8_kernel<float, 128, WRITE, 4>, kv8_kernel<float, 128, WRITE, 1>);
   } else {
-    if (c->head_dim == 64) hipLaunchKernelGGL((kv8_kernel<uint16_t, 64, WRITE>), g, b, 0, s, a);
-    else hipLaunchKernelGGL((kv8_kernel<uint16_t, 128, WRITE>), g, b, 0, s, a);
+    if (c->head_dim == 64) go(kv8_kernel<uint16_t, 64, WRITE, 4>, kv8_kernel<uint16_t, 64, WRITE, 1>);
+    else go(kv8_kernel<uint16_t, 128, WRITE, 4>, kv8_kernel<uint16_t, 128, WRITE, 1>);
   }
   return itts::check_launch(fn);
 }
