@@ -471,6 +471,10 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
       load(tile + 32 * kWaves);
       if (LINEAGE && tile + 64 * kWaves < end) load_rows(tile + 64 * kWaves);
     }
+    // the columns' scores, scaled (a.qk_scale > 0), and their maxima; all columns go through each stage together, so that
+    // one's products cover another's latencies
+    float x[NQ][8], top[NQ];
+    bool grow = rescale != 1.f;
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
       f32x4_t s[2];
@@ -484,25 +488,33 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
             s[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kf[f][e]),
                                                            __builtin_bit_cast(bf16x8_t, qf[j][e][q]), s[f], 0, 0, 0);
       }
-      float x[8];
-      uint32_t vis = 0xFF;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) x[u] = s[u >> 2][u & 3];
-      if (any_bad) {
+      for (int u = 0; u < 8; ++u) x[j][u] = s[u >> 2][u & 3] * a.qk_scale;
+    }
+    if (any_bad) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) x[u] = bad >> u & 1 ? __builtin_nanf("") : x[u];
+      for (int j = 0; j < NQ; ++j)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[j][u] = bad >> u & 1 ? __builtin_nanf("") : x[j][u];
+    }
+    if (edge) {
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        const uint32_t vis = mine(prefix_bits(tile) | drafted_bits(tile, msk[j]));
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[j][u] = vis >> u & 1 ? x[j][u] : -__builtin_inff();
       }
-      if (edge) {
-        vis = mine(prefix_bits(tile) | drafted_bits(tile, msk[j]));
+    }
 #pragma unroll
-        for (int u = 0; u < 8; ++u) x[u] = vis >> u & 1 ? x[u] : -__builtin_inff();
-      }
-      float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-      top = top * a.qk_scale;  // positive
-
-      top = max_rows(top);
-      if (__any(top > m[j] + kLag) || rescale != 1.f) {
-        const float next = fmaxf(m[j], top);
+    for (int j = 0; j < NQ; ++j) {
+      top[j] = max_rows(fmaxf(fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])),
+                              fmaxf(fmaxf(x[j][4], x[j][5]), fmaxf(x[j][6], x[j][7]))));
+      grow |= top[j] > m[j] + kLag;
+    }
+    if (__any(grow)) {
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        const float next = fmaxf(m[j], top[j]);
         const float f = next == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m[j] - next);
         m[j] = next;
         l[j] = l[j] * f;
@@ -510,13 +522,13 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[j][d] = o[j][d] * fo;
       }
+    }
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
       float p[8];
       const float shift = (float)kPUp - (m[j] == -__builtin_inff() ? 0.f : m[j]);
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float z = fmaf(x[u], a.qk_scale, shift);
-        p[u] = __builtin_amdgcn_exp2f(z);
-      }
+      for (int u = 0; u < 8; ++u) p[u] = __builtin_amdgcn_exp2f(x[j][u] + shift);
 #pragma unroll
       for (int q = 0; q < PN; ++q) {
         u32x4_t pf;
