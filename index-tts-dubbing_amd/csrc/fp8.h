@@ -8,10 +8,6 @@
 
 namespace itts {
 
-constexpr float kE4m3Max = 448.f;  // 1.75 * 2^8
-
-__device__ __forceinline__ bool finite_f(float x) { return fabsf(x) < __builtin_inff(); }
-
 // scale byte of a block whose largest finite magnitude is a: E = min { e : a <= 1.75 * 2^(8 + e) }, e >= -126
 __device__ __forceinline__ int e4m3_scale_byte(float a) {
   const uint32_t u = __float_as_uint(a);
@@ -26,10 +22,6 @@ __device__ __forceinline__ float e4m3_scale(int byte) { return __uint_as_float((
 __device__ __forceinline__ uint32_t e4m3_pack4(float a, float b, float c, float d) {
   int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
-}
-// v * inv, with what is not finite as NaN
-__device__ __forceinline__ float e4m3_prescale(float v, float inv) {
-  return finite_f(v) ? v * inv : __builtin_nanf("");
 }
 
 // The magnitudes' maximum is taken on their bits: as integers they order like the values, and what is not finite comes out

@@ -621,9 +621,10 @@ __global__ __launch_bounds__(256, 1) void fp8_linear_large_kernel(LinearArgs p) 
 }
 
 // ---- few rows ----
-// 16 columns of y and MT x 16 rows per workgroup; its eight waves take the blocks of k in turn and add their parts in LDS.
-// x is quantised on the way (a lane holds 32 of a row's 128 values; four lanes share the block), so there is one launch
-// and no workspace; w's fragments come straight from global memory: with few rows the bytes of w are the cost.
+// 16 columns of y and MT x 16 rows per workgroup; its eight waves take the blocks of k in turn and add their parts in LDS, in
+// wave order.  With few rows the bytes of w and the latency of fetching them are the cost.  x comes as codes, or as values
+// that are quantised on the way (a lane holds 32 of a row's 128 values; four lanes share the block): one launch and no
+// workspace.
 constexpr int kFewWaves = 8;
 
 // 32 values of a row as they come from memory: chunks k .. +15 and k + 64 .. +79
@@ -677,87 +678,146 @@ struct Raw32 {
   }
 };
 
+// the lane's 32 values as codes, and their block's scale
+template <typename T>
+__device__ __forceinline__ i32x8_t codes(const Raw32<T>& raw, int& scale) {
+  float v[32];
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[16 * g + i] = raw.value(g, i);
+  auto reduce = [](uint32_t m) {  // the four lanes of the row
+    m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+    return max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+  };
+  scale = itts::e4m3_scaled(v, reduce(raw.max_bits()), reduce);
+  i32x8_t f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = (int)e4m3_pack4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  return f;
+}
+
+// T: bf16 or f32 values, or codes (with their scales in p).  A wave's blocks of w (and of codes) go to its own part of the
+// LDS by DMA, two slots in turn, in the layout of the tile kernels: the matrix unit wants neighbouring lanes on neighbouring
+// rows, and the load path handles such lanes one by one (59 accesses per load instruction; fetched to registers that way,
+// 96 x 4096 x 1024 took 13.2 us instead of 8.2).
 template <bool EXACT, typename T, int MT>
 __global__ __launch_bounds__(64 * kFewWaves) void fp8_linear_few_kernel(LinearArgs p, const T* __restrict__ x, int64_t ldx, int K, bool vec) {
+  constexpr bool CODES = std::is_same_v<T, uint8_t>;
+  constexpr int DMA = 2 + (CODES ? 2 * MT : 0);  // instructions of 8 rows: w's 16, then x's
+  constexpr int SLOT = 1024 * DMA;
+  __shared__ __attribute__((aligned(1024))) uint8_t s0[kFewWaves * SLOT], s1[kFewWaves * SLOT];
+  __shared__ f32x4_t part[kFewWaves][MT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, c = lane >> 4;
   const int n0 = blockIdx.x * 16;
   const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
-  const uint8_t* wr = p.wq + (int64_t)min(n0 + r, p.N - 1) * p.ldw + 16 * c;
+  const uint8_t* src[DMA];
+#pragma unroll
+  for (int i = 0; i < DMA; ++i) {
+    const int row = 8 * i + (lane >> 3), chunk = 16 * ((lane & 7) ^ (row >> 1 & 7));
+    src[i] = (i < 2 ? p.wq + (int64_t)min(n0 + row, p.N - 1) * p.ldw : p.xq + min(m0 + row - 16, p.M - 1) * p.ldxq) + chunk;
+  }
+  auto issue = [&](int kb, uint8_t* slot) {
+#pragma unroll
+    for (int i = 0; i < DMA; ++i)
+      __builtin_amdgcn_global_load_lds(static_cast<const void*>(src[i] + 128 * kb), (lds_void*)(slot + SLOT * wave + 1024 * i), 16, 0, 0);
+  };
+  const int nb = (p.KB - wave + kFewWaves - 1) / kFewWaves;  // this wave's blocks: wave + 8 i
+  if (nb > 0) issue(wave, s0);
+  // scale bytes of four of the wave's blocks at a time, lane group c those of block i + c
   const uint8_t* wsr = p.ws + (int64_t)min(n0 + r, p.N - 1) * p.ldws;
+  const uint8_t* xsr[MT];
   const T* xr[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
-    const int64_t m = m0 + 16 * t + r;
-    xr[t] = x + (m < p.M ? m : p.M - 1) * ldx;
+    const int64_t m = min(m0 + 16 * t + r, p.M - 1);
+    xr[t] = x + m * ldx;
+    xsr[t] = p.xs + m * p.ldxs;
   }
+  int ws4 = 0, xs4[MT];
+  auto load_scales = [&](int i) {
+    const int kb = min(wave + kFewWaves * (i + c), p.KB - 1);
+    ws4 = wsr[kb];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) xs4[t] = CODES ? xsr[t][kb] : 0;
+  };
+  load_scales(0);
+  Raw32<T> raw[CODES ? 1 : MT];
+  auto load_raw = [&](int kb) {
+    if constexpr (!CODES) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) raw[t].load(xr[t], 128 * kb + 16 * c, K, vec);
+    }
+  };
+  if (nb > 0) load_raw(wave);
+  // bias and residual of the one result that this thread adds up
+  static_assert(MT <= 2, "one result per thread");
+  const int row = threadIdx.x >> 4, col = threadIdx.x & 15;
+  const bool mine = row < 16 * MT && m0 + row < p.M && n0 + col < p.N;
+  const float bias = p.bias && mine ? p.bias[n0 + col] : 0.f;
+  const float residual = p.residual && mine ? p.residual[(m0 + row) * p.ldr + n0 + col] : 0.f;
+
   f32x4_t acc[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  // the next block's operands are requested before this one's are used
-  i32x8_t wn;
-  int sn;
-  Raw32<T> xn[MT];
-  auto fetch = [&](int kb) {
-    wn = frag(wr + kb * 128);
-    sn = wsr[kb];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) xn[t].load(xr[t], 128 * kb + 16 * c, K, vec);
+  const int a0 = r * 128 + ((c ^ (r >> 1 & 7)) << 4), a1 = r * 128 + (((4 + c) ^ (r >> 1 & 7)) << 4);
+  auto read = [&](const uint8_t* s) -> i32x8_t {
+    const u32x4_t lo = *reinterpret_cast<const u32x4_t*>(s + a0), hi = *reinterpret_cast<const u32x4_t*>(s + a1);
+    return i32x8_t{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
   };
-  if (wave < p.KB) fetch(wave);
-  for (int kb = wave; kb < p.KB; kb += kFewWaves) {
-    const i32x8_t wf = wn;
-    const int sw = sn;
-    Raw32<T> xc[MT];
+  auto step = [&](int i, uint8_t* slot, uint8_t* other) {
+    const uint8_t* s = slot + SLOT * wave;
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): the block has landed, this wave's reads of the other slot are done
+    asm volatile("" ::: "memory");
+    Raw32<T> now[CODES ? 1 : MT];
+    if constexpr (!CODES) {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) xc[t] = xn[t];
-    if (kb + kFewWaves < p.KB) fetch(kb + kFewWaves);
+      for (int t = 0; t < MT; ++t) now[t] = raw[t];
+    }
+    const int at = r + 16 * (i & 3);
+    const int sw = __shfl(ws4, at, 64);
+    int sx[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) sx[t] = CODES ? __shfl(xs4[t], at, 64) : 0;
+    if (i + 1 < nb) {
+      issue(wave + kFewWaves * (i + 1), other);
+      load_raw(wave + kFewWaves * (i + 1));
+      if (((i + 1) & 3) == 0) load_scales(i + 1);
+    }
+    const i32x8_t wf = read(s);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      float v[32];
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[16 * g + i] = xc[t].value(g, i);
-      auto reduce = [](uint32_t m) {  // the four lanes of the row
-        m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
-        return max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-      };
-      const int sx = itts::e4m3_scaled(v, reduce(xc[t].max_bits()), reduce);
       i32x8_t xf;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) xf[i] = (int)e4m3_pack4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      if constexpr (CODES) xf = read(s + 2048 * (1 + t));
+      else xf = codes(now[t], sx[t]);
       if constexpr (EXACT) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(dequant8(wf[2 * e], wf[2 * e + 1], itts::e4m3_scale(sw)),
-                                                           dequant8(xf[2 * e], xf[2 * e + 1], itts::e4m3_scale(sx)), acc[t], 0, 0, 0);
+                                                           dequant8(xf[2 * e], xf[2 * e + 1], itts::e4m3_scale(sx[t])), acc[t], 0, 0, 0);
       } else {
-        acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf, acc[t], 0, 0, 0, sw, 0, sx);
+        acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf, acc[t], 0, 0, 0, sw, 0, sx[t]);
       }
     }
+  };
+  for (int i = 0; i < nb; i += 2) {
+    step(i, s0, s1);
+    if (i + 1 < nb) step(i + 1, s1, s0);
   }
-  __shared__ f32x4_t part[kFewWaves][MT][64];
 #pragma unroll
   for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
   __syncthreads();
-  // 16 MT rows x 16 columns over the threads, columns fastest
-  for (int i = threadIdx.x; i < MT * 256; i += 64 * kFewWaves) {
-    const int row = i >> 4, col = i & 15;
-    const int t = row >> 4, src = (col >> 2) * 16 + (row & 15);
-    float v = 0.f;
+  if (!mine) return;
+  float v = bias;
 #pragma unroll
-    for (int w = 0; w < kFewWaves; ++w) v += part[w][t][src][col & 3];
-    const int64_t m = m0 + row;
-    const int n = n0 + col;
-    if (m < p.M && n < p.N) {
-      v += p.bias ? p.bias[n] : 0.f;
-      v = p.act == 0 ? v : p.act == 1 ? apply_act<1>(v) : apply_act<2>(v);
-      if (p.residual) v += p.residual[m * p.ldr + n];
-      if (p.out_bf16) ((uint16_t*)p.y)[m * p.ldy + n] = f2bf(v);
-      else ((float*)p.y)[m * p.ldy + n] = v;
-    }
-  }
+  for (int w = 0; w < kFewWaves; ++w) v += part[w][row >> 4][(col >> 2) * 16 + (row & 15)][col & 3];
+  v = p.act == 0 ? v : p.act == 1 ? apply_act<1>(v) : apply_act<2>(v);
+  v += residual;
+  const int64_t at = (m0 + row) * p.ldy + n0 + col;
+  if (p.out_bf16) ((uint16_t*)p.y)[at] = f2bf(v);
+  else ((float*)p.y)[at] = v;
 }
 
 int launch_quant(const char* fn, const void* x, int64_t ldx, int dtype, int64_t M, int K, uint8_t* q, int64_t ldq,
@@ -779,13 +839,19 @@ int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 int64_t code_pitch(int K) { return round_up(K, 128); }
 int64_t scale_pitch(int K) { return round_up(round_up(K, 128) / 128, 4); }
 
-// Few rows: one launch of the small kernel, whose rate (it quantises x once per 16 columns of y) is some 90 TFLOP/s, against a
-// quantising pass and tiles.  Measured, us (this / 128 x 128 tiles): 96 x 4096 x 1024 17 / 44, 96 x 1024 x 4096 15 / 16,
-// 300 x 1024 x 1024 14 / 15, 2000 x 1024 x 4096 195 / 22.
-bool few_rows(int64_t M, int N, int K) { return M <= 32 || M * N * (int64_t)K <= 500000000; }
+// x quantised within the product (one launch, no workspace) while that is done by few: with more rows or a long k the
+// same values are quantised once per 16 columns of y.  Measured, us (this / quantised first): 1 x 1024 x 4096 3.3 / 5.8,
+// 16 x 4096 x 1024 6.6 / 7.7, 32 x 1024 x 4096 5.5 / 5.8, 32 x 2048 x 1024 6.9 / 6.2, 32 x 4096 x 1024 10.8 / 7.7.
+bool few_rows(int64_t M, int K) { return M <= 16 || (M <= 32 && K <= 1024); }
+// 32 x 16 outputs per workgroup with k split among its waves, while that is at most three turns of the 256 CUs: a 128 x 128
+// tile takes 0.8 us per block of k, one after the other.  Measured, us (this / such tiles, both with the quantising pass of
+// 2.5): 96 x 4096 x 1024 8.2 / 29, 96 x 1024 x 4096 10.0 / 12.2, 300 x 1024 x 1024 10.0 / 12.4, 800 x 256 x 2048 25 / 8.7.
+bool some_rows(int64_t M, int N) { return ((M + 31) / 32) * ((N + 15) / 16) <= 768; }
 // 256 x 256 tiles once they keep most of the 256 CUs busy (and the scales of all of k fit the LDS beside them).  Measured,
 // us (these / 128 x 128): 14400 x 1024 x 4096 107 / 122, 8192 x 8192 x 8192 467 / 657, 2000 x 1024 x 4096 (128 tiles) 26 / 22.
-bool large_tiles(int64_t M, int N, int K) { return ((M + 255) / 256) * ((N + 255) / 256) >= 200 && K <= 128 * kScaleBlocks; }
+bool large_tiles(int64_t M, int N, int K) {
+  return M > 128 && N > 128 && ((M + 255) / 256) * ((N + 255) / 256) >= 200 && K <= 128 * kScaleBlocks;
+}
 
 template <bool EXACT, int BM, int BN, int WM, int WN>
 void launch_tile(const LinearArgs& p, hipStream_t st) {
@@ -800,22 +866,12 @@ void launch_large(const LinearArgs& p, hipStream_t st) {
   else if (p.act == 1) hipLaunchKernelGGL(fp8_linear_large_kernel<1>, g, b, 0, st, p);
   else hipLaunchKernelGGL(fp8_linear_large_kernel<2>, g, b, 0, st, p);
 }
-#ifndef VAR
-#define VAR 0
-#endif
-template <typename T>
+template <typename T, int MT>
 void launch_few(const T* x, int64_t ldx, int K, bool vec, const LinearArgs& p, hipStream_t st) {
-  const int mt = p.M <= 16 ? 1 : 2;
-  const dim3 g((p.N + 15) / 16, (unsigned)((p.M + 16 * mt - 1) / (16 * mt))), b(64 * kFewWaves);
-  if (p.out_bf16) {
-    if (mt == 1) hipLaunchKernelGGL((fp8_linear_few_kernel<false, T, 1>), g, b, 0, st, p, x, ldx, K, vec);
-    else hipLaunchKernelGGL((fp8_linear_few_kernel<false, T, 2>), g, b, 0, st, p, x, ldx, K, vec);
-  } else {
-    if (mt == 1) hipLaunchKernelGGL((fp8_linear_few_kernel<true, T, 1>), g, b, 0, st, p, x, ldx, K, vec);
-    else hipLaunchKernelGGL((fp8_linear_few_kernel<true, T, 2>), g, b, 0, st, p, x, ldx, K, vec);
-  }
+  const dim3 g((p.N + 15) / 16, (unsigned)((p.M + 16 * MT - 1) / (16 * MT))), b(64 * kFewWaves);
+  if (p.out_bf16) hipLaunchKernelGGL((fp8_linear_few_kernel<false, T, MT>), g, b, 0, st, p, x, ldx, K, vec);
+  else hipLaunchKernelGGL((fp8_linear_few_kernel<true, T, MT>), g, b, 0, st, p, x, ldx, K, vec);
 }
-
 }  // namespace
 
 extern "C" int itts_fp8_quant_rows(const void* x, int64_t ldx, int x_dtype, int64_t M, int K, uint8_t* q, int64_t ldq,
@@ -832,7 +888,7 @@ extern "C" int itts_fp8_quant_rows(const void* x, int64_t ldx, int x_dtype, int6
 
 extern "C" int64_t itts_fp8_linear_workspace_bytes(int64_t M, int N, int K) {
   if (M < 0 || N < 1 || N > kMaxN || K < 1 || K > kMaxK || M > ((int64_t)1 << 40) / code_pitch(K)) return -1;
-  return few_rows(M, N, K) ? 0 : round_up(M, 256) * (code_pitch(K) + scale_pitch(K));  // whole tiles of rows
+  return few_rows(M, K) ? 0 : round_up(M, 256) * (code_pitch(K) + scale_pitch(K));  // whole tiles of rows
 }
 
 extern "C" int itts_fp8_linear(const void* x, int64_t ldx, int x_dtype, int64_t M, int K, const uint8_t* wq, int64_t ldw,
@@ -848,7 +904,7 @@ extern "C" int itts_fp8_linear(const void* x, int64_t ldx, int x_dtype, int64_t 
                    ldws <= kMaxK,
                fn, "weight rows need K rounded up to 128 bytes, scale rows ceil(K / 128) rounded up to 4");
   if (M == 0) return 0;
-  const bool few = few_rows(M, N, K);
+  const bool few = few_rows(M, K);
   ITTS_REQUIRE(x && wq && ws && y && (few || workspace), fn, "null pointer");
   ITTS_REQUIRE((((uintptr_t)wq | (uintptr_t)workspace) & 15) == 0 && ((uintptr_t)ws & 3) == 0, fn, "misaligned pointer");
   ITTS_REQUIRE(((M + 127) / 128) * ((N + 127) / 128) <= 0x7FFFFFFF, fn, "too many tiles for one launch");
@@ -861,12 +917,15 @@ extern "C" int itts_fp8_linear(const void* x, int64_t ldx, int x_dtype, int64_t 
                    ((uintptr_t)bias & 15) == 0 && ((uintptr_t)residual & 15) == 0 && (!residual || ldr % 4 == 0)};
   if (few) {
     const bool vec = ((uintptr_t)x & 15) == 0 && ldx % (x_dtype == ITTS_F32 ? 4 : 8) == 0;
-    if (x_dtype == ITTS_F32) launch_few((const float*)x, ldx, K, vec, p, st);
-    else launch_few((const uint16_t*)x, ldx, K, vec, p, st);
+    if (x_dtype == ITTS_F32 && M <= 16) launch_few<float, 1>((const float*)x, ldx, K, vec, p, st);
+    else if (x_dtype == ITTS_F32) launch_few<float, 2>((const float*)x, ldx, K, vec, p, st);
+    else if (M <= 16) launch_few<uint16_t, 1>((const uint16_t*)x, ldx, K, vec, p, st);
+    else launch_few<uint16_t, 2>((const uint16_t*)x, ldx, K, vec, p, st);
     return itts::check_launch(fn);
   }
   if (int rc = launch_quant(fn, x, ldx, x_dtype, M, K, xq, code_pitch(K), xs, scale_pitch(K), st)) return rc;
-  if (!p.out_bf16) launch_tile<true, 128, 128, 64, 64>(p, st);
+  if (some_rows(M, N)) launch_few<uint8_t, 2>(xq, p.ldxq, K, true, p, st);
+  else if (!p.out_bf16) launch_tile<true, 128, 128, 64, 64>(p, st);
   else if (large_tiles(M, N, K)) launch_large(p, st);
   else launch_tile<false, 128, 128, 64, 64>(p, st);
   return itts::check_launch(fn);

@@ -73,7 +73,7 @@ def oracle(x, w, bias, act, residual, fast):
 
 def check(got, y, tol):
     half = torch.finfo(got.dtype).eps / 2
-    err = (got.cpu().double() - y).abs()
+    err = (got.to(y.device).double() - y).abs()
     assert torch.isfinite(got).all()
     assert bool((err <= tol + half * (y.abs() + tol) + 1e-30).all()), float((err / (tol + half * y.abs() + 1e-30)).max())
 
@@ -177,3 +177,76 @@ def test_linear_captured(M):
         torch.cuda.synchronize()
         got = y.clone()
         assert torch.equal(got, layer(x, act=1)), i
+
+
+# more rows x columns than 32 x 16 outputs of a workgroup can take in three turns: 128 x 128 tiles; sides and reductions that
+# end inside a tile, one to 65 blocks of k (the scales of 64 are held at once)
+TILES = [(51300, 129, 16), (9, 1100, 51300), (1000, 1, 400), (2100, 130, 200), (3333, 300, 144), (1537, 512, 1000), (700, 8200, 640)]
+# from 200 tiles of 256 x 256 on, bf16 results: those
+LARGE = [(3500, 100, 3600), (3500, 256, 3601), (3585, 300, 3600), (3499, 640, 3700), (51300, 129, 200), (151, 1100, 51300),
+         (3500, 8192, 3600)]
+
+
+BF16_FORMS = ["gelu", "bf16", "bf16 residual"]
+
+
+@pytest.mark.parametrize("M,K,N,form", [(*s, f) for s in TILES + LARGE for f in BF16_FORMS] +
+                         [(*s, f) for s in TILES for f in ("plain", "silu", "residual")])
+def test_linear_tiles(M, K, N, form):
+    from indextts.utils.fp8 import Fp8Linear
+    fast = form in BF16_FORMS
+    g = torch.Generator(device="cuda").manual_seed(M * 7 + K + N)
+    x = torch.randn(M, K, generator=g, device="cuda") * torch.exp2(torch.randint(-3, 4, (1, K), generator=g, device="cuda").float())
+    x = x.bfloat16() if fast else x
+    w = torch.randn(N, K, generator=g, device="cuda") / K ** 0.5
+    bias = None if form == "silu" else torch.randn(N, generator=g, device="cuda") * 0.3
+    res = torch.randn(M, N, generator=g, device="cuda") if "residual" in form else None
+    act = {"gelu": 1, "silu": 2}.get(form, 0)
+    got = Fp8Linear.from_weight(w, bias)(x, act=act, residual=res, bf16_out=fast)
+    check(got, *oracle(x, w, bias, act, res, fast))
+
+
+@pytest.mark.parametrize("M,K,N,fast", [(1100, 512, 1024, False), (1100, 512, 1024, True), (3500, 512, 3600, True)])
+def test_tiles_scales_far_apart_and_not_finite(M, K, N, fast):
+    from indextts.utils.fp8 import Fp8Linear
+    g = torch.Generator(device="cuda").manual_seed(6)
+
+    def spread(rows):
+        e = torch.exp2(torch.randint(-20, 20, (rows, K // 128), generator=g, device="cuda").float())
+        return torch.randn(rows, K, generator=g, device="cuda") * e.repeat_interleave(128, 1)
+    x, w = spread(M), spread(N)
+    check(Fp8Linear.from_weight(w)(x, bf16_out=fast), *oracle(x, w, None, 0, None, fast))
+    x[3, 7], x[M - 1, 200], w[11, 3] = float("nan"), float("inf"), float("nan")
+    bad = torch.zeros(M, N, dtype=torch.bool, device="cuda")
+    bad[3], bad[M - 1], bad[:, 11] = True, True, True
+    assert torch.equal(torch.isnan(Fp8Linear.from_weight(w)(x, bf16_out=fast)), bad)
+
+
+def test_many_rows_of_a_narrow_layer():
+    """more rows than 65535 workgroups of 32"""
+    from indextts.utils.fp8 import Fp8Linear
+    g = torch.Generator(device="cuda").manual_seed(8)
+    w = torch.randn(8, 16, generator=g, device="cuda")
+    layer = Fp8Linear.from_weight(w, torch.randn(8, generator=g, device="cuda"))
+    x = torch.randn(2200001, 16, generator=g, device="cuda")
+    y = layer(x)
+    for at in (slice(0, 9), slice(2097144, 2097160), slice(2199990, 2200001)):
+        check(y[at], *oracle(x[at], w, layer.bias, 0, None, False))
+
+
+@pytest.mark.parametrize("M,N,fast", [(1100, 1024, False), (1100, 1024, True), (3500, 3600, True)])
+def test_tiles_captured(M, N, fast):
+    from indextts.utils.fp8 import Fp8Linear
+    g = torch.Generator(device="cuda").manual_seed(9)
+    layer = Fp8Linear.from_weight(torch.randn(N, 300, generator=g, device="cuda"))
+    x = torch.randn(M, 300, generator=g, device="cuda")
+    layer(x, bf16_out=fast)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = layer(x, act=2, bf16_out=fast)
+    for i in range(4):
+        x.copy_(torch.randn(M, 300, generator=g, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, layer(x, act=2, bf16_out=fast))
