@@ -69,13 +69,16 @@ __device__ __forceinline__ void store4(const AttnArgs& a, int64_t at, f32x4_t y)
   }
 }
 
+// larger of two scores as the median with the largest float (an infinite score makes its column NaN all the same): fmaxf
+// first brings both into canonical form, two more instructions, which cost 64 tokens x 4 heads over 16301 keys 7 us of 124
+__device__ __forceinline__ float max2(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, 3.4028234663852886e38f); }
 // max over the four lanes that hold a column: lanes l, l ^ 16, l ^ 32, l ^ 48
 __device__ __forceinline__ float max_rows(float v) {
   const uint32_t u = __float_as_uint(v);
   const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  const uint32_t w = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+  const uint32_t w = __float_as_uint(max2(__uint_as_float(a[0]), __uint_as_float(a[1])));
   const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+  return max2(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ int max_rows(int v) {
   const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
@@ -426,23 +429,24 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
     float sv[8];
     float rescale = 1.f;
     if constexpr (E4M3) {
-      int vs[8];
+      int vs[8];  // the scales as f32 bits, which order like them
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        vs[u] = tvs[u >> 2] >> (8 * (u & 3)) & 0xFF;
+        const uint32_t w = tvs[u >> 2];
+        vs[u] = ((u & 3) == 3 ? w >> 1 : w << (23 - 8 * (u & 3))) & 0x7F800000u;
       }
       if (edge) {  // what nothing is seen of has no part in the reference; its V is 0
 #pragma unroll
         for (int u = 0; u < 8; ++u) vs[u] = some >> u & 1 ? vs[u] : 0;
       }
       int top = max(max(max(vs[0], vs[1]), max(vs[2], vs[3])), max(max(vs[4], vs[5]), max(vs[6], vs[7])));
-      top = __builtin_amdgcn_readfirstlane(max_rows(top));  // 16 lanes each hold the same eight bytes
+      top = __builtin_amdgcn_readfirstlane(max_rows(top)) >> 23;  // 16 lanes each hold the same eight bytes
       if (top > vref) {
         rescale = vref == 0 ? 0.f : __builtin_amdgcn_exp2f((float)(vref - top));
         vref = top;
       }
 #pragma unroll
-      for (int u = 0; u < 8; ++u) sv[u] = __uint_as_float((uint32_t)max(vs[u] - vref + 127 + kVUp, 0) << 23);
+      for (int u = 0; u < 8; ++u) sv[u] = __builtin_ldexpf(__uint_as_float(vs[u]), 127 + kVUp - vref);
     }
     u32x4_t vf[DT], kf[2][KS];
     v_frags(tv, sv, vf);
@@ -471,7 +475,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
       load(tile + 32 * kWaves);
       if (LINEAGE && tile + 64 * kWaves < end) load_rows(tile + 64 * kWaves);
     }
-    // the columns' scores, scaled (a.qk_scale > 0), and their maxima; all columns go through each stage together, so that
+    // the columns' scores and their maxima (a.qk_scale > 0); all columns go through each stage together, so that
     // one's products cover another's latencies
     float x[NQ][8], top[NQ];
     bool grow = rescale != 1.f;
@@ -489,7 +493,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
                                                            __builtin_bit_cast(bf16x8_t, qf[j][e][q]), s[f], 0, 0, 0);
       }
 #pragma unroll
-      for (int u = 0; u < 8; ++u) x[j][u] = s[u >> 2][u & 3] * a.qk_scale;
+      for (int u = 0; u < 8; ++u) x[j][u] = s[u >> 2][u & 3];
     }
     if (any_bad) {
 #pragma unroll
@@ -507,8 +511,8 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
     }
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
-      top[j] = max_rows(fmaxf(fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])),
-                              fmaxf(fmaxf(x[j][4], x[j][5]), fmaxf(x[j][6], x[j][7]))));
+      top[j] = max_rows(max2(max2(max2(x[j][0], x[j][1]), max2(x[j][2], x[j][3])),
+                             max2(max2(x[j][4], x[j][5]), max2(x[j][6], x[j][7]))) * a.qk_scale);
       grow |= top[j] > m[j] + kLag;
     }
     if (__any(grow)) {
@@ -528,7 +532,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
       float p[8];
       const float shift = (float)kPUp - (m[j] == -__builtin_inff() ? 0.f : m[j]);
 #pragma unroll
-      for (int u = 0; u < 8; ++u) p[u] = __builtin_amdgcn_exp2f(x[j][u] + shift);
+      for (int u = 0; u < 8; ++u) p[u] = __builtin_amdgcn_exp2f(fmaf(x[j][u], a.qk_scale, shift));
 #pragma unroll
       for (int q = 0; q < PN; ++q) {
         u32x4_t pf;
