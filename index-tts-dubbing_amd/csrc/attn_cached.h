@@ -1,7 +1,7 @@
 // Attention of one new token (itts_attn_decode_kv8) or of a tree of drafted tokens (itts_attn_tree) per row over a KV
 // cache in block-scaled e4m3 (fp8.h) or bf16.
 //
-// One wave walks its share of a row and K/V head's keys in tiles of 32, with up to NQ x 16 query columns (column = drafted
+// One wave walks its share of a row and K/V head's keys in tiles of 32, with NQ x 16 query columns (column = drafted
 // token * group + query head of the group), everything in registers:
 //   S^T [32 keys][columns] = K Q^T     (A = K, B = Q^T; v_mfma_f32_16x16x32_bf16, two per 32 dims)
 //   running maximum and sum per column (a column's keys lie in the lanes l, l ^ 16, l ^ 32, l ^ 48)
@@ -92,8 +92,8 @@ constexpr int kWaves = 4;  // waves of a workgroup take its tiles in turn
 // waves per SIMD that the registers are held to: the most that leave the loop without spills
 template <bool E4M3, bool LINEAGE, int HD, int QN, int NQ>
 constexpr int waves_per_simd() {
-  if (E4M3 && HD == 64) return NQ == 1 ? 3 : NQ == 2 ? (QN == 1 && !LINEAGE ? 3 : 2) : (QN == 1 ? 2 : 1);
-  if (E4M3 || HD == 64) return NQ == 1 || (NQ == 2 && QN == 1 && !LINEAGE) ? 2 : 1;
+  if (E4M3 && HD == 64) return NQ == 1 || (QN == 1 && !LINEAGE) ? 3 : 2;
+  if (E4M3 || HD == 64) return NQ == 1 || (QN == 1 && !LINEAGE) ? 2 : 1;
   return 1;
 }
 
@@ -623,9 +623,48 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
   }
 }
 
-// launches of one element type and head size, over the query tiles (attn_cached_*.hip)
+// ---- launches, by the types and the query tiles (attn_cached_*.hip hold the instances) ----
+// Columns of 16 that a wave takes at once.  Two share a tile's loads and conversions; four (64 dims) spill or run at one wave
+// per SIMD, and so do two of 128 dims with an f32 q.  Measured, us (one / two / four): 32 x 16 heads, 64 tokens over 600 keys
+// of 64 dims 27 / 24 / 24, f32 q 33 / 30 / 45, bf16 cache 39 / 29 / 40; 4 x 8 heads x 4, 64 tokens over 16000 keys of 128 dims
+// 189 / 120 / -, f32 q 191 / 197 / -; 8 x 8 heads x 4, 8 tokens over 4000 keys of 128 dims 23.5 / 25.4 / -, f32 q 25 / 36 / -.
+inline int query_tiles(bool e4m3, int cols, bool q_f32, int hd) {
+  if (cols <= 16) return 1;
+  return e4m3 && hd == 128 && (q_f32 || cols <= 32) ? 1 : 2;
+}
+
+template <bool E4M3, bool LINEAGE, int HD, int QN, int PN, int NQ>
+void launch_one(const AttnArgs& a, hipStream_t s) {
+  const int64_t us = ((int64_t)a.units * a.nsplit + 7) / 8 * 8;
+  hipLaunchKernelGGL((attn_cached_kernel<E4M3, LINEAGE, HD, QN, PN, NQ>), dim3((unsigned)(us * a.qblocks)),
+                     dim3(64 * kWaves), 0, s, a);
+}
+template <bool E4M3, bool LINEAGE, int HD, int QN, int PN>
+void launch_nq(const AttnArgs& a, hipStream_t s) {
+  constexpr bool ONE = E4M3 && HD == 128 && QN == 3;
+  if (ONE || query_tiles(E4M3, a.T * a.G, a.q_f32, HD) == 1) launch_one<E4M3, LINEAGE, HD, QN, PN, 1>(a, s);
+  else if constexpr (!ONE) launch_one<E4M3, LINEAGE, HD, QN, PN, 2>(a, s);
+}
+// bf16 V takes P as two parts, e4m3 V for f32 outputs alone
+template <bool E4M3, bool LINEAGE, int HD>
+void launch_types(const AttnArgs& a, hipStream_t s) {
+  if (a.q_f32) {
+    if (!E4M3 || a.out_f32) launch_nq<E4M3, LINEAGE, HD, 3, 2>(a, s);
+    else if constexpr (E4M3) launch_nq<E4M3, LINEAGE, HD, 3, 1>(a, s);
+  } else {
+    if (!E4M3 || a.out_f32) launch_nq<E4M3, LINEAGE, HD, 1, 2>(a, s);
+    else if constexpr (E4M3) launch_nq<E4M3, LINEAGE, HD, 1, 1>(a, s);
+  }
+}
 template <bool E4M3, int HD>
-void launch_attn(const AttnArgs& a, int nq, hipStream_t s);
+void launch_attn(const AttnArgs& a, hipStream_t s);
 
 }  // namespace attn
 }  // namespace itts
+
+#define ITTS_ATTN_CACHED_INSTANCES(E4M3, HD)                                   \
+  template <>                                                                  \
+  void itts::attn::launch_attn<E4M3, HD>(const AttnArgs& a, hipStream_t s) {   \
+    if (a.kv_rows) launch_types<E4M3, true, HD>(a, s);                         \
+    else launch_types<E4M3, false, HD>(a, s);                                  \
+  }

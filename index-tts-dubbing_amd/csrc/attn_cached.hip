@@ -67,15 +67,14 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   store4(a, (int64_t)b * a.o_sb + t * a.o_st + (int64_t)(h * a.G + cg - t * a.G) * a.o_sh + d, acc * inv);
 }
 
-// columns of 16 that one wave takes at once, by their number and what fits the registers
-// dims: two)
-int query_tiles(int cols, bool q_f32, int hd) { return cols <= 16 ? 1 : cols <= 32 || hd == 128 ? 2 : 4; }
-int query_blocks(int cols, bool q_f32, int hd) {
-  const int per = 16 * query_tiles(cols, q_f32, hd);
+int query_blocks(bool e4m3, int cols, bool q_f32, int hd) {
+  const int per = 16 * query_tiles(e4m3, cols, q_f32, hd);
   return (cols + per - 1) / per;
 }
 // Splits over the keys: enough workgroups for two on each of the 256 CUs, none with fewer than 512 keys of the expected
-// longest row (each wave then has four tiles to keep the next one's loads in flight).
+// longest row (each wave then has four tiles to keep the next one's loads in flight).  Measured, us (kernel + join, with 512
+// / 1024 / 2048 workgroups wanted): 8 x 4 heads over 32749 keys 46 + 5 / 46 + 7 / 52 + 11, 64 tokens of 4 x 8 heads over
+// 16301 keys 125 + 6 / 124 + 7 / 139 + 9; 32 x 16 heads over 565 keys unsplit 14, in two 17 + 6.
 int splits(int64_t workgroups, int max_len) {
   const int64_t want = (512 + workgroups - 1) / (workgroups > 0 ? workgroups : 1);
   const int64_t most = (max_len + 511) / 512;
@@ -88,7 +87,7 @@ int attend(const char* fn, AttnArgs& a, int B, int q_dtype, int out_dtype, int m
                "out must be bf16, or f32 over an e4m3 cache");
   const int64_t need = itts_attn_cached_workspace_bytes(&a.c, B, a.T, a.G, max_len, q_dtype);
   ITTS_REQUIRE(need >= 0, fn, "bad sizes (1 <= T <= 64, 1 <= group <= 4096, rows x heads x query blocks of one launch)");
-  ITTS_REQUIRE(a.kv_rows ? a.ld_rows >= a.c.max_kv || B <= 1 : B <= a.c.rows, fn,
+  ITTS_REQUIRE(a.kv_rows ? a.ld_rows >= a.c.max_kv : B <= a.c.rows, fn,
                "more rows than the cache holds, or a short lineage table");
   ITTS_REQUIRE(a.qk_scale == a.qk_scale && a.qk_scale - a.qk_scale == 0.f, fn, "the scale must be finite");
   if (B == 0) return 0;
@@ -101,18 +100,17 @@ int attend(const char* fn, AttnArgs& a, int B, int q_dtype, int out_dtype, int m
   a.q_vec = ((uintptr_t)a.q & 15) == 0 && ((a.q_sb | a.q_st | a.q_sh) * qs) % 16 == 0;
   a.o_vec = ((uintptr_t)a.out & 15) == 0 && ((a.o_sb | a.o_st | a.o_sh) * os) % 16 == 0;
   a.units = B * a.c.heads;
-  a.qblocks = query_blocks(cols, a.q_f32, hd);
+  a.qblocks = query_blocks(a.c.dtype == ITTS_E4M3, cols, a.q_f32, hd);
   a.nsplit = splits((int64_t)a.units * a.qblocks, max_len);
   a.part = (float*)workspace;
   a.part_ml = a.part + (int64_t)a.units * a.nsplit * cols * hd;
-  const int nq = query_tiles(cols, a.q_f32, hd);
   hipStream_t s = itts::as_stream(stream);
   if (a.c.dtype == ITTS_E4M3) {
-    if (hd == 64) launch_attn<true, 64>(a, nq, s);
-    else launch_attn<true, 128>(a, nq, s);
+    if (hd == 64) launch_attn<true, 64>(a, s);
+    else launch_attn<true, 128>(a, s);
   } else {
-    if (hd == 64) launch_attn<false, 64>(a, nq, s);
-    else launch_attn<false, 128>(a, nq, s);
+    if (hd == 64) launch_attn<false, 64>(a, s);
+    else launch_attn<false, 128>(a, s);
   }
   if (a.nsplit > 1) {
     const unsigned g = (unsigned)(((int64_t)a.units * cols + 3) / 4);
@@ -129,7 +127,7 @@ extern "C" int64_t itts_attn_cached_workspace_bytes(const ItTsKvCache* c, int B,
       group > 4096 || max_len < 0 || (q_dtype != ITTS_F32 && q_dtype != ITTS_BF16))
     return -1;
   const int64_t units = (int64_t)B * c->heads, cols = (int64_t)T * group;
-  const int qblocks = query_blocks((int)cols, q_dtype == ITTS_F32, c->head_dim);
+  const int qblocks = query_blocks(c->dtype == ITTS_E4M3, (int)cols, q_dtype == ITTS_F32, c->head_dim);
   const int nsplit = splits(units * qblocks, max_len);
   if ((units * nsplit + 7) * qblocks > 0x7FFFFF00 || units * cols > 0x7FFFFF00) return -1;
   return nsplit > 1 ? units * nsplit * cols * (c->head_dim + 2) * 4 : 0;

@@ -3,8 +3,9 @@
 // scale bytes [row][head][pos].
 //
 // Pure traffic: a token and head reads hd values and writes hd + 1 bytes for each of K and V.  hd / 8 lanes per vector,
-// eight values per lane, so a lane's 16-B (bf16) or 32-B (f32) load becomes one 8-B store.  What it needs is loads in
-// flight: KVNOTE
+// eight values per lane, so a lane's 16-B (bf16) or 32-B (f32) load becomes one 8-B store.  A head's values of one token are a
+// piece of hd bytes somewhere in the cache, so what bounds it is the latency of scattered pieces, not arithmetic: 24000 tokens
+// of 16 heads x 64 in bf16 take 42 us to write and 45 to read (147 MB each, 3.4 TB/s; a large copy reaches 5); 32 tokens 3.
 #include "fp8.h"
 
 namespace {
@@ -146,7 +147,8 @@ int launch(const char* fn, const ItTsKvCache* c, const void* k, int64_t k_st, in
   ITTS_REQUIRE(k && v && row && pos, fn, "null pointer");
   const int es = dtype == ITTS_F32 ? 4 : 2;
   const bool vec = (((uintptr_t)k | (uintptr_t)v) & 15) == 0 && ((k_st | k_sh | v_st | v_sh) * es) % 16 == 0;
-  // four tokens a lane where that leaves workgroups enough, one where latency counts
+  // Four tokens a lane where that leaves workgroups enough, one where latency counts.  Measured, us (one / four): 32 tokens
+  // written 3.1 / 4.7, 4096 read 7.9 / 7.5, 24000 written 29.1 / 27.3 and read 29.2 / 27.9 (slots in order).
   const int turns = M >= 4096 ? 4 : 1;
   const int group = (c->heads + 7) / 8;
   const int64_t lanes = (int64_t)group * 2 * (c->head_dim / 8);
