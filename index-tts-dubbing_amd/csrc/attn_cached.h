@@ -16,6 +16,12 @@
 // (2^-31 of it at the least: smaller ones round), P enters as f16 in [0, 2^15] (half step 2^-12 of a weight, below the
 // bf16 output's 2^-9) or, for f32 outputs, as two f16 parts (2^-23).  bf16 V: P as two bf16 parts (2^-17).
 // Maxima, sums and both products accumulate in f32.
+//
+// What bounds it, and what it takes (kernel time): few tokens over long rows run at the memory's rate (8 rows x 4 heads, up to
+// 32749 keys of 128 dims: 216 MB in 45 us = 4.8 TB/s, and 5 us to join the splits); with lineage tables (96 rows x 16 heads,
+// up to 483 keys of 64 dims) it is the tables' and addresses' arithmetic, 28 us for 78 MB; short rows cost a launch and one
+// trip to memory (131 keys: 5.8 us); many columns (64 tokens x 4 heads, 16301 keys: 116 us for 27 GFLOP, 112 MB) the vector
+// instructions around the products, some 350 per 32 keys and 32 columns, half of them K's and V's conversion.
 #pragma once
 #include "fp8.h"
 
@@ -70,7 +76,8 @@ __device__ __forceinline__ void store4(const AttnArgs& a, int64_t at, f32x4_t y)
 }
 
 // larger of two scores as the median with the largest float (an infinite score makes its column NaN all the same): fmaxf
-// first brings both into canonical form, two more instructions, which cost 64 tokens x 4 heads over 16301 keys 7 us of 124
+// first brings both into canonical form, two more instructions each (with V's scales as f32 bits 4 us of 120
+// for 64 tokens x 4 heads over 16301 keys)
 __device__ __forceinline__ float max2(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, 3.4028234663852886e38f); }
 // max over the four lanes that hold a column: lanes l, l ^ 16, l ^ 32, l ^ 48
 __device__ __forceinline__ float max_rows(float v) {

@@ -7,6 +7,10 @@
 // 13 bits below it (measured on normal data: 1.5e-5 of the result's rms; the bf16 result rounds by 1.7e-3).
 // f32 outputs: codes times scale are exact in bf16, and v_mfma_f32_16x16x32_bf16 adds exact products to f32 (measured
 // 1.2e-8 of the rms), at half the rate and one conversion per two codes.
+//
+// What bounds it (times with the quantising pass): few rows the launch and the trip to memory (1 x 1024 x 4096: 3.3 us for
+// 4.3 MB, 96 x 4096 x 1024: 8.2); large sizes the matrix unit (8192 x 8192 x 8192: 449 us = 2.45 PFLOP/s) less the tiles' first
+// fetch and last store (14400 x 1024 x 4096 with GELU: 104 us = 1.16 PFLOP/s, four turns of 256 tiles of eight steps each).
 #include <type_traits>
 
 #include "fp8.h"
@@ -197,7 +201,7 @@ __device__ __forceinline__ void store_direct(const LinearArgs& p, f32x4_t (&acc)
 }
 
 // Any N and pitch: bands of 16 rows go through the wave's own part of the LDS, then lanes walk the rows with neighbouring
-// columns, so that whole lines are written all the same (57 us instead of 101 at 1337 x 1000 x 8194).
+// columns, so that whole lines are written all the same (stored from the registers, 1337 x 1000 x 8194 took 44 us more).
 template <bool BF16, bool AGPR, int ACT, bool RES, int FM, int FN>
 __device__ __forceinline__ void store_banded(const LinearArgs& p, f32x4_t (&acc)[FM][FN], float* band, int64_t m0, int n0) {
   constexpr int WN = 16 * FN, CI = WN / 64;
@@ -848,9 +852,10 @@ bool few_rows(int64_t M, int K) { return M <= 16 || (M <= 32 && K <= 1024); }
 // 2.5): 96 x 4096 x 1024 8.2 / 29, 96 x 1024 x 4096 10.0 / 12.2, 300 x 1024 x 1024 10.0 / 12.4, 800 x 256 x 2048 25 / 8.7.
 bool some_rows(int64_t M, int N) { return ((M + 31) / 32) * ((N + 15) / 16) <= 768; }
 // 256 x 256 tiles once they keep most of the 256 CUs busy (and the scales of all of k fit the LDS beside them).  Measured,
-// us (these / 128 x 128): 14400 x 1024 x 4096 107 / 122, 8192 x 8192 x 8192 467 / 657, 2000 x 1024 x 4096 (128 tiles) 26 / 22.
+// us with the quantising pass (these / 128 x 128): 14400 x 1024 x 4096 93 / 114, 14400 x 4096 x 1024 84 / 102, 8192 x 8192 x
+// 8192 449 / 644, 3000 x 1024 x 4096 (192 tiles) 27 / 30, 2000 x 1024 x 4096 (128 tiles) 25 / 21.
 bool large_tiles(int64_t M, int N, int K) {
-  return M > 128 && N > 128 && ((M + 255) / 256) * ((N + 255) / 256) >= 200 && K <= 128 * kScaleBlocks;
+  return M > 128 && N > 128 && ((M + 255) / 256) * ((N + 255) / 256) >= 160 && K <= 128 * kScaleBlocks;
 }
 
 template <bool EXACT, int BM, int BN, int WM, int WN>

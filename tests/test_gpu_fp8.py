@@ -182,7 +182,7 @@ def test_linear_captured(M):
 # more rows x columns than 32 x 16 outputs of a workgroup can take in three turns: 128 x 128 tiles; sides and reductions that
 # end inside a tile, one to 65 blocks of k (the scales of 64 are held at once)
 TILES = [(51300, 129, 16), (9, 1100, 51300), (1000, 1, 400), (2100, 130, 200), (3333, 300, 144), (1537, 512, 1000), (700, 8200, 640)]
-# from 200 tiles of 256 x 256 on, bf16 results: those
+# from 160 tiles of 256 x 256 on, bf16 results: those
 LARGE = [(3500, 100, 3600), (3500, 256, 3601), (3585, 300, 3600), (3499, 640, 3700), (51300, 129, 200), (151, 1100, 51300),
          (3500, 8192, 3600)]
 
