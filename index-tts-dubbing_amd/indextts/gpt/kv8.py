@@ -51,11 +51,12 @@ class _Cache:
         self._ref = ctypes.byref(self._c)
         self.scale = hd ** -0.5
         self.lib = _hip.load()
+        self._need = {}  # workspace bytes by the sizes of a call
 
     def _index(self, t: Optional[torch.Tensor], n: int, name: str) -> Optional[int]:
         if t is None:
             return None
-        if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous() or t.get_device() != self.index:
+        if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous() or t.get_device() != self.index:
             raise ValueError(f"{name} must be a contiguous int32 tensor of {n} on {self.dev}")
         return t.data_ptr()
 
@@ -79,9 +80,14 @@ class _Cache:
         return group
 
     def _workspace(self, B, T, group, max_len, q_dtype):
-        n = self.lib.itts_attn_cached_workspace_bytes(self._ref, B, T, group, max_len, q_dtype)
-        if n < 0:
-            raise ValueError("sizes the attention does not take (T <= 64, group <= 4096)")
+        n = self._need.get((B, T, group, max_len, q_dtype))
+        if n is None:
+            n = self.lib.itts_attn_cached_workspace_bytes(self._ref, B, T, group, max_len, q_dtype)
+            if n < 0:
+                raise ValueError("sizes the attention does not take (T <= 64, group <= 4096)")
+            if len(self._need) >= 4096:
+                self._need.clear()
+            self._need[B, T, group, max_len, q_dtype] = n
         return torch.empty(n, dtype=torch.uint8, device=self.dev) if n else None
 
     def tree(self, q: torch.Tensor, kv_len: torch.Tensor, mask: torch.Tensor, n_tokens: Optional[torch.Tensor] = None,
@@ -146,9 +152,9 @@ class Kv8Cache(_Cache):
         (row[i], pos[i]), int32 [M].  A slot outside the cache is skipped (-1 for a padding token); the slots of one
         call must differ from each other."""
         shape = k.shape
-        if len(shape) != 3 or v.shape != shape or v.dtype != k.dtype or self._heads(k, shape, "k") != 1 or \
-                self._heads(v, shape, "v") != 1:
-            raise ValueError(f"k and v must be [M, {self.heads}, {self.head_dim}], alike")
+        if len(shape) != 3 or self._heads(k, shape, "k") != 1 or v.shape != shape or v.dtype != k.dtype or \
+                v.stride(2) != 1 or v.get_device() != self.index:
+            raise ValueError(f"k and v must be [M, {self.heads}, {self.head_dim}], alike, on {self.dev}")
         M, ks, vs = shape[0], k.stride(), v.stride()
         rc = self.lib.itts_kv8_write(self._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _CODE[k.dtype],
                                      self._index(row, M, "row"), self._index(pos, M, "pos"), M,
@@ -162,9 +168,9 @@ class Kv8Cache(_Cache):
         code = _CODE.get(dtype)
         if code is None or row.dim() != 1:
             raise ValueError("dtype must be f32 or bf16, row [M]")
-        M, H, hd = row.shape[0], self.heads, self.head_dim
-        kv = torch.empty((2, M, H, hd), dtype=dtype, device=self.dev)
-        k, v = kv.unbind(0)
+        M, H, hd = row.numel(), self.heads, self.head_dim
+        shape = (M, H, hd)
+        k, v = self.k.new_empty(shape, dtype=dtype), self.k.new_empty(shape, dtype=dtype)
         rc = self.lib.itts_kv8_read(self._ref, self._index(row, M, "row"), self._index(pos, M, "pos"), M, k.data_ptr(), H * hd,
                                     hd, v.data_ptr(), H * hd, hd, code, _hip.current_stream_of(self.index))
         if rc:
@@ -184,7 +190,7 @@ class Kv8Cache(_Cache):
         group = self._heads(q, shape, "q")
         B = shape[0]
         if out is None:
-            out = torch.empty(shape, dtype=dtype, device=self.dev)
+            out = q.new_empty(shape, dtype=dtype)
         elif out.shape != shape or out.stride(2) != 1 or out.get_device() != self.index:
             raise ValueError(f"out must be {tuple(shape)} with unit last stride on {self.dev}")
         qd, od = _CODE[q.dtype], _CODE.get(out.dtype)

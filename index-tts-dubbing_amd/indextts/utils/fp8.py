@@ -7,6 +7,7 @@ weight bytes and twice the matrix rate, at e4m3's half step of 2^-4 per value.
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -15,6 +16,11 @@ from .. import _hip
 
 BLOCK = 128
 _CODE = {torch.float32: _hip.F32, torch.bfloat16: _hip.BF16}
+
+
+@lru_cache(4096)
+def _workspace_bytes(M: int, N: int, K: int) -> int:
+    return _hip.load().itts_fp8_linear_workspace_bytes(M, N, K)
 
 
 def quant_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -88,7 +94,7 @@ class Fp8Linear:
             ldx = K
         dt, yd = (torch.bfloat16, _hip.BF16) if bf16_out else (torch.float32, _hip.F32)
         if out is None:
-            y = torch.empty(ys, dtype=dt, device=self.dev)
+            y = x.new_empty(ys, dtype=dt)
         else:
             y = out
             if y.dtype != dt or y.shape != ys or not y.is_contiguous() or y.get_device() != dev:
@@ -101,8 +107,8 @@ class Fp8Linear:
             res = residual.data_ptr()
         if M == 0:
             return y
-        n = self.lib.itts_fp8_linear_workspace_bytes(M, N, K)
-        ws = torch.empty(n, dtype=torch.uint8, device=self.dev) if n > 0 else None
+        n = _workspace_bytes(M, N, K)
+        ws = x.new_empty(n, dtype=torch.uint8) if n > 0 else None
         wq, ldw, wsc, lds, b = self._w
         rc = self.lib.itts_fp8_linear(x.data_ptr(), ldx, xd, M, K, wq, ldw, wsc, lds, N, b, act, res, N, y.data_ptr(), N, yd,
                                       None if ws is None else ws.data_ptr(), _hip.current_stream_of(dev))
