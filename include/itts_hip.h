@@ -574,7 +574,8 @@ int itts_attn_decode_kv8(const ItTsKvCache* c, const void* q, int64_t q_sb, int6
  * (n = n_tokens[b], NULL: T).  Token t sees p in [pad[b], kv_len[b]) and the drafted token j wherever bit j of
  * mask[b * mask_sb + t] is set (its ancestors and itself; any set of bits is allowed, bits >= n are ignored; mask_sb
  * 0: one tree for all rows).  What a token does not see does not reach it, NaN included; a token that sees nothing
- * gives 0.  Outputs of tokens >= n are left as they were.  kv_len < 0, n outside 0 .. T or kv_len + n > max_kv: the
+ * gives 0, one that sees only scores of -inf NaN; an infinite V before kv_len gives infinity or NaN in its dimension.
+ * Outputs of tokens >= n are left as they were.  kv_len < 0, n outside 0 .. T or kv_len + n > max_kv: the
  * row's T outputs are NaN.  The rest as itts_attn_decode_kv8; over a bf16 cache out is bf16. */
 int itts_attn_tree(const ItTsKvCache* c, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int q_dtype, int B,
                    int T, int group, const int32_t* kv_len, const int32_t* pad, const int32_t* n_tokens,

@@ -79,6 +79,15 @@ __device__ __forceinline__ void store4(const AttnArgs& a, int64_t at, f32x4_t y)
 // first brings both into canonical form, two more instructions each (with V's scales as f32 bits 4 us of 120
 // for 64 tokens x 4 heads over 16301 keys)
 __device__ __forceinline__ float max2(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, 3.4028234663852886e38f); }
+// 1 / the sum of a token's weights, for an output: a row that sees nothing gives 0; where every score that it sees is -inf there
+// is no weight to divide by, and the result is NaN
+__device__ __forceinline__ float inverse_sum(const AttnArgs& a, float sum, int b, int t, int len, int n) {
+  if (sum != 0.f) return 1.f / sum;
+  bool sees = (a.pad ? max(a.pad[b], 0) : 0) < len;
+  if (a.tree) sees |= (a.mask[(int64_t)b * a.mask_sb + t] & (n < 64 ? (1ull << n) - 1 : ~0ull)) != 0;
+  return sees ? __builtin_nanf("") : 0.f;
+}
+
 // max over the four lanes that hold a column: lanes l, l ^ 16, l ^ 32, l ^ 48
 __device__ __forceinline__ float max_rows(float v) {
   const uint32_t u = __float_as_uint(v);
@@ -96,11 +105,13 @@ __device__ __forceinline__ int max_rows(int v) {
 
 constexpr int kWaves = 4;  // waves of a workgroup take its tiles in turn
 
-// waves per SIMD that the registers are held to: the most that leave the loop without spills
+// waves per SIMD that the registers are held to: the most that leave the loop without spills (32 x 16 heads, 64 tokens with an
+// f32 q over 600 keys of a bf16 cache: 36 us at two, 56 at one)
 template <bool E4M3, bool LINEAGE, int HD, int QN, int NQ>
 constexpr int waves_per_simd() {
   if (E4M3 && HD == 64) return NQ == 1 || (QN == 1 && !LINEAGE) ? 3 : 2;
-  if (E4M3 || HD == 64) return NQ == 1 || (QN == 1 && !LINEAGE) ? 2 : 1;
+  if (HD == 64) return 2;
+  if (E4M3) return NQ == 1 || (QN == 1 && !LINEAGE) ? 2 : 1;
   return 1;
 }
 
@@ -486,21 +497,44 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
     // one's products cover another's latencies
     float x[NQ][8], top[NQ];
     bool grow = rescale != 1.f;
+    auto scores = [&](const u32x4_t (&low)[2][KS]) {  // low: what the lower parts of q meet
 #pragma unroll
-    for (int j = 0; j < NQ; ++j) {
-      f32x4_t s[2];
+      for (int j = 0; j < NQ; ++j) {
+        f32x4_t s[2];
 #pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        s[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int f = 0; f < 2; ++f) {
+          s[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < KS; ++e)
+          for (int e = 0; e < KS; ++e)
 #pragma unroll
-          for (int q = QN - 1; q >= 0; --q)
-            s[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kf[f][e]),
-                                                           __builtin_bit_cast(bf16x8_t, qf[j][e][q]), s[f], 0, 0, 0);
+            for (int q = QN - 1; q >= 0; --q)
+              s[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, q ? low[f][e] : kf[f][e]),
+                                                             __builtin_bit_cast(bf16x8_t, qf[j][e][q]), s[f], 0, 0, 0);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[j][u] = s[u >> 2][u & 3];
       }
+    };
+    scores(kf);
+    if constexpr (!E4M3 && QN > 1) {  // an infinite K times a lower part of 0 is NaN: once more without such products
+      bool nan = false;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) x[j][u] = s[u >> 2][u & 3];
+      for (int j = 0; j < NQ; ++j)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) nan |= x[j][u] != x[j][u];
+      if (__any(nan)) {
+        u32x4_t low[2][KS];
+#pragma unroll
+        for (int f = 0; f < 2; ++f)
+#pragma unroll
+          for (int e = 0; e < KS; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t w = kf[f][e][i];
+              low[f][e][i] = w & ~(((((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u) >> 15) * 0xFFFFu);
+            }
+        scores(low);
+      }
     }
     if (any_bad) {
 #pragma unroll
@@ -624,7 +658,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
     } else {
       const int t = cg / G;
       if (!refuse && t >= nt) continue;
-      const float inv = refuse ? __builtin_nanf("") : sum == 0.f ? 0.f : vscale / sum;
+      const float inv = refuse ? __builtin_nanf("") : vscale * inverse_sum(a, sum, b, t, len, n);
       store4(a, (int64_t)b * a.o_sb + t * a.o_st + (int64_t)(h * G + cg - t * G) * a.o_sh + d, acc * inv);
     }
   }

@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], o, 64);
   }
   if (g != 0) return;
-  const float inv = refuse ? __builtin_nanf("") : sum == 0.f ? 0.f : 1.f / sum;
+  const float inv = refuse ? __builtin_nanf("") : inverse_sum(a, sum, b, t, len, n);
   store4(a, (int64_t)b * a.o_sb + t * a.o_st + (int64_t)(h * a.G + cg - t * a.G) * a.o_sh + d, acc * inv);
 }
 

@@ -363,6 +363,60 @@ def test_tree_refuses_rows_it_cannot_read():
     assert torch.isnan(got[1][see]).all() and torch.equal(got[1][~see], good[1][~see])
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("T,heads,group", [(5, 2, 1), (33, 1, 2)])
+@pytest.mark.parametrize("e4m3,q_dtype,out_dtype", TYPES)
+@pytest.mark.parametrize("longest", [200, 1300])
+def test_tree_lineage(hd, T, heads, group, e4m3, q_dtype, out_dtype, longest):
+    """keys, drafted ones too, from rows that a table names; in one part and split over the keys"""
+    lens = [0, 3, 190, 64, 129]
+    c, k, v, q, mask = tree_case(5, T, heads, group, hd, lens, 51, e4m3, q_dtype)
+    g = torch.Generator().manual_seed(52)
+    S = k.shape[2]
+    kv_rows = torch.randint(5, (5, S + 2), generator=g).int().cuda()
+    pad, n = i32([0, 0, 66, 64, 1]), i32([T, 2, T, 1, T - 1])
+    out = torch.zeros(q.shape, dtype=out_dtype, device="cuda")
+    got = c.tree(q, i32(lens), mask, n_tokens=n, pad=pad, kv_rows=kv_rows, max_len=longest, out=out)
+    at = kv_rows[:, :S].long()[:, None], torch.arange(heads, device="cuda")[None, :, None], torch.arange(S, device="cuda")[None, None]
+    see = seen_keys(5, T, S, i32(lens), pad, mask, n) & (torch.arange(T)[None] < n.cpu()[:, None])[:, :, None]
+    check_rows(got, q, k[at], v[at], see, hd ** -0.5, pieces(q_dtype, out_dtype, e4m3), out_dtype)
+
+
+@pytest.mark.parametrize("e4m3,q_dtype,out_dtype", TYPES)
+@pytest.mark.parametrize("hd,T,heads,group", [(64, 3, 2, 1), (64, 40, 1, 1), (128, 3, 1, 4), (128, 12, 1, 4)])
+def test_tree_long(e4m3, q_dtype, out_dtype, hd, T, heads, group):
+    """split over the keys, with short rows beside a long one; a drafted value that is not finite in the last part"""
+    lens = [2490, 3, 700, 0]
+    c, k, v, q, mask = tree_case(4, T, heads, group, hd, lens, 61, e4m3, q_dtype)
+    got = c.tree(q, i32(lens), mask, dtype=out_dtype)
+    check_rows(got, q, k, v, seen_keys(4, T, k.shape[2], i32(lens), None, mask), hd ** -0.5, pieces(q_dtype, out_dtype, e4m3), out_dtype)
+    c.v[0, 0, 2491, 3] = 0x7F if e4m3 else float("nan")
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[0, :, :group, 3] = (mask[0] >> 1 & 1).bool()[:, None]
+    again = c.tree(q, i32(lens), mask, dtype=out_dtype)
+    assert torch.equal(torch.isnan(again), bad) and torch.equal(torch.where(bad, 0, again), torch.where(bad, 0, got))
+
+
+@pytest.mark.parametrize("longest", [70, 1300])
+def test_tree_infinite_scores(longest):
+    """a key whose score is -inf has no weight; where a token sees no other key the result is NaN, where it sees none 0"""
+    from indextts.gpt.kv8 import Kv16Cache
+    g = torch.Generator().manual_seed(71)
+    k, v = (torch.randn(4, 1, 80, 64, generator=g).bfloat16().cuda() for _ in range(2))
+    k[:, :, :, 0] = 0
+    q = torch.randn(4, 2, 1, 64, generator=g).cuda()
+    q[..., 0] = 1.0
+    k[0, 0, 5, 0] = float("-inf")
+    k[1, 0, :60, 0] = float("-inf")
+    k[2, 0, 7, 0] = float("inf")
+    got = Kv16Cache(k, v).tree(q, i32([60, 60, 60, 0]), torch.tensor([0, 2], device="cuda"), max_len=longest)
+    assert torch.isnan(got[1, 0]).all() and torch.isnan(got[2]).all() and (got[3, 0] == 0).all()
+    see = seen_keys(4, 2, 80, i32([60, 60, 60, 0]), None, torch.tensor([0, 2]))
+    see[0, :, 5], see[1, :, :60], see[2] = False, False, False
+    check_rows(torch.where(torch.isnan(got), 0, got), q, torch.nan_to_num(k.double(), posinf=0, neginf=0), v.double(), see, 0.125,
+               BF16_P2, torch.bfloat16)
+
+
 def test_tree_of_one_token_is_decode():
     c, k, v = filled(4, 2, 90, 64)
     q = torch.randn(4, 6, 64, device="cuda")
