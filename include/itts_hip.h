@@ -527,7 +527,7 @@ int itts_gpt_decode_steps_pl(const ItTsGptWeights* w, const ItTsGptPlLayerW* pl,
 int itts_fp8_quant_rows(const void* x, int64_t ldx, int x_dtype, int64_t M, int K, uint8_t* q, int64_t ldq, uint8_t* s,
                         int64_t lds, void* stream);
 /* y [M][N] = act(Q(x) Q(w)^T + bias) + residual: x [M][K] f32 or bf16 is quantised within the call, w comes
- * quantised (itts_fp8_quant_rows), bias [N] f32 and residual [M][ldr] f32 optional (residual may be y itself),
+ * quantised (itts_fp8_quant_rows), bias [N] f32 and residual [M][ldr] f32 optional (residual may be y itself; y must not overlap x),
  * act 0 none, 1 gelu_tanh, 2 SiLU (as itts_igemm_fwd), y f32 (exact products, f32 accumulation) or bf16 (the 8-bit
  * matrix unit: f32 accumulation of 128 products at a time, which it aligns to the largest of them).  A row's result does
  * not depend on the other rows' values; workspace: itts_fp8_linear_workspace_bytes (0: none needed), 16-B aligned,
@@ -565,7 +565,7 @@ int64_t itts_attn_cached_workspace_bytes(const ItTsKvCache* c, int B, int T, int
  * (optional, max_kv entries a row): key p of row b is read from cache row kv_rows[b * ld_rows + p] (the lineage table of
  * itts_attn_decode_rows); an entry outside the cache makes that row's output NaN.  kv_len outside 0 .. max_kv: NaN.
  * max_len: the largest kv_len the caller expects (it sizes the split over keys; larger ones stay right).
- * q f32 or bf16, out bf16 or f32 (strides in elements, unit head_dim stride). */
+ * q f32 or bf16, out bf16 or f32 (strides in elements, unit head_dim stride); out must not overlap q or the cache. */
 int itts_attn_decode_kv8(const ItTsKvCache* c, const void* q, int64_t q_sb, int64_t q_sh, int q_dtype, int B, int group,
                          const int32_t* kv_len, const int32_t* pad, const int32_t* kv_rows, int64_t ld_rows, float scale,
                          int max_len, void* out, int64_t o_sb, int64_t o_sh, int out_dtype, void* workspace, void* stream);

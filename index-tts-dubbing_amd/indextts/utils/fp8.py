@@ -78,7 +78,7 @@ class Fp8Linear:
     def __call__(self, x: torch.Tensor, act: int = 0, residual: Optional[torch.Tensor] = None, bf16_out: bool = False,
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """act(x @ W^T + b) (+ residual); act 0 none, 1 gelu_tanh, 2 SiLU; y f32, or bf16 with ``bf16_out``;
-        residual f32 [..., N], contiguous, may be ``out`` itself."""
+        residual f32 [..., N], contiguous, may be ``out`` itself; ``out`` must not overlap x."""
         K, N, dev = self.in_features, self.out_features, self.index
         shape = x.shape
         xd = _CODE.get(x.dtype)
@@ -99,6 +99,9 @@ class Fp8Linear:
             y = out
             if y.dtype != dt or y.shape != ys or not y.is_contiguous() or y.get_device() != dev:
                 raise ValueError(f"out must be a contiguous {dt} tensor of {ys} on {self.dev}")
+            if M and x.data_ptr() < y.data_ptr() + M * N * y.element_size() and \
+                    y.data_ptr() < x.data_ptr() + ((M - 1) * ldx + K) * x.element_size():
+                raise ValueError("out must not overlap x: other columns of a row still read it")
         res = None
         if residual is not None:
             if residual.dtype != torch.float32 or residual.shape != ys or not residual.is_contiguous() or \

@@ -250,3 +250,15 @@ def test_tiles_captured(M, N, fast):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, layer(x, act=2, bf16_out=fast))
+
+
+def test_out_over_x_is_refused():
+    from indextts.utils.fp8 import Fp8Linear
+    layer = Fp8Linear.from_weight(torch.randn(128, 128, device="cuda"))
+    x = torch.randn(40, 128, device="cuda")
+    for out in (x, x[3:13]):
+        with pytest.raises(ValueError):
+            layer(x[:out.shape[0]] if out is not x else x, out=out)
+    both = torch.randn(80, 128, device="cuda")
+    want = layer(both[:40])
+    assert torch.equal(layer(both[:40], out=both[40:]), want) and torch.equal(both[40:], want)
