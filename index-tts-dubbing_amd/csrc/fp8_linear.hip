@@ -121,7 +121,7 @@ struct LinearArgs {
 template <int WN>
 constexpr int kPitch = WN + 4;  // floats: rows r and r + 1 four banks apart
 template <int WN>
-constexpr int kBand = 16 * kPitch<WN> * 4;  // bytes of a wave's band
+constexpr int kBand = 2 * (WN / 64) * 16 * (64 * 4 + 16);  // bytes of a wave's part of the LDS; 16 rows of kPitch floats fit too
 
 // A sum as a vector register.  AGPR: it stays in its accumulator register until here (left to itself the compiler copies a
 // wave's 256 sums at once, and spills).
@@ -137,11 +137,14 @@ __device__ __forceinline__ f32x4_t sums_of(f32x4_t a) {
   return f32x4_t{sum_of<AGPR>(a[0]), sum_of<AGPR>(a[1]), sum_of<AGPR>(a[2]), sum_of<AGPR>(a[3])};
 }
 
-// N a multiple of 16 and aligned rows: a lane's 16 neighbouring results from registers, the four lane groups' 64 side by
-// side.  A row's residual is requested before the stores of the row before (a load waits for the stores before it).
+// N a multiple of 16 and aligned rows: a lane has 16 neighbouring results of a row.  They go through the wave's own part of
+// the LDS in their final type, so that neighbouring lanes store neighbouring 16 bytes (stored from where they are, neighbouring
+// lanes on neighbouring rows, a store takes the load / store path 64 clocks instead of 16: XXNOTE).  A row's residual is
+// requested before the stores of the row before (a load waits for the stores before it).
 template <bool BF16, bool AGPR, int ACT, bool RES, int FM, int FN>
-__device__ __forceinline__ void store_direct(const LinearArgs& p, f32x4_t (&acc)[FM][FN], int64_t m0, int n0) {
-  constexpr int G = FN / 4;
+__device__ __forceinline__ void store_direct(const LinearArgs& p, f32x4_t (&acc)[FM][FN], uint8_t* band, int64_t m0, int n0) {
+  constexpr int G = FN / 4, ES = BF16 ? 2 : 4;
+  constexpr int PITCH = 64 * ES + 16, CHUNKS = 4 * ES;  // a row's 64 results in the LDS; 16-B pieces of them
   const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
   const int left = (int)(p.M - m0 < 16 * FM ? p.M - m0 : 16 * FM);  // rows of the wave's tile
   f32x4_t bias[G][4], res[RES ? G : 1][4];
@@ -181,21 +184,29 @@ __device__ __forceinline__ void store_direct(const LinearArgs& p, f32x4_t (&acc)
         if constexpr (RES) v[g][j] = v[g][j] + res[g][j];
       }
     if (i + 1 < FM) load_res(i + 1);
+    uint8_t* const buf = band + (i & 1) * (G * 16 * PITCH);
 #pragma unroll
     for (int g = 0; g < G; ++g)
-      if (in[g] && row < left) {
-        const int64_t at = (m0 + row) * p.ldy + n0 + 64 * g + 16 * c;
-        if constexpr (BF16) {
-          u32x4_t* d = reinterpret_cast<u32x4_t*>((uint16_t*)p.y + at);
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            d[h] = u32x4_t{pack2bf(v[g][2 * h][0], v[g][2 * h][1]), pack2bf(v[g][2 * h][2], v[g][2 * h][3]),
-                           pack2bf(v[g][2 * h + 1][0], v[g][2 * h + 1][1]), pack2bf(v[g][2 * h + 1][2], v[g][2 * h + 1][3])};
-        } else {
-          f32x4_t* d = reinterpret_cast<f32x4_t*>((float*)p.y + at);
+      for (int k = 0; k < ES; ++k) {
+        u32x4_t w;
+        if constexpr (BF16)
+          w = u32x4_t{pack2bf(v[g][2 * k][0], v[g][2 * k][1]), pack2bf(v[g][2 * k][2], v[g][2 * k][3]),
+                      pack2bf(v[g][2 * k + 1][0], v[g][2 * k + 1][1]), pack2bf(v[g][2 * k + 1][2], v[g][2 * k + 1][3])};
+        else
+          w = __builtin_bit_cast(u32x4_t, v[g][k]);
+        *reinterpret_cast<u32x4_t*>(buf + (16 * g + r) * PITCH + 16 * ES * c + 16 * k) = w;
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the band is this wave's own: no barrier
 #pragma unroll
-          for (int j = 0; j < 4; ++j) d[j] = v[g][j];
-        }
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int k = 0; k < ES; ++k) {
+        const int at = 64 / CHUNKS * k + lane / CHUNKS, chunk = lane % CHUNKS;
+        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(buf + (16 * g + at) * PITCH + 16 * chunk);
+        const int col = n0 + 64 * g + chunk * (16 / ES);
+        if (16 * i + at < left && col < p.N)
+          *reinterpret_cast<u32x4_t*>((uint8_t*)p.y + ((m0 + 16 * i + at) * p.ldy + col) * ES) = w;
       }
   }
 }
@@ -247,8 +258,8 @@ template <bool BF16, bool AGPR, int ACT, int FM, int FN>
 __device__ __forceinline__ void store_tile(const LinearArgs& p, f32x4_t (&acc)[FM][FN], float* band, int64_t m0, int n0) {
   if (m0 >= p.M) return;
   if (p.vec_out) {
-    if (p.residual) store_direct<BF16, AGPR, ACT, true>(p, acc, m0, n0);
-    else store_direct<BF16, AGPR, ACT, false>(p, acc, m0, n0);
+    if (p.residual) store_direct<BF16, AGPR, ACT, true>(p, acc, (uint8_t*)band, m0, n0);
+    else store_direct<BF16, AGPR, ACT, false>(p, acc, (uint8_t*)band, m0, n0);
   } else {
     if (p.residual) store_banded<BF16, AGPR, ACT, true>(p, acc, band, m0, n0);
     else store_banded<BF16, AGPR, ACT, false>(p, acc, band, m0, n0);
@@ -277,7 +288,7 @@ __device__ __forceinline__ bf16x8_t dequant8(int lo, int hi, float scale) {
 // fragment read lie on distinct banks; the DMA writes lane by lane, so each lane fetches the chunk that belongs where it
 // writes.  W is the A operand: a lane's results are W rows at one row of x.  The 64 W rows of a wave's four fragments are
 // dealt as 16 (r / 4) + 4 j + r % 4 (fragment j, row r), which makes a lane's 16 results 16 consecutive columns of y and
-// the four lane groups' 64: whole lines are written without going through LDS.
+// the four lane groups' 64.
 typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kScaleBlocks = 64;  // blocks of k whose scales the LDS holds at once
@@ -620,6 +631,7 @@ __global__ __launch_bounds__(256, 1) void fp8_linear_large_kernel(LinearArgs p) 
   __builtin_amdgcn_s_waitcnt(0x0070);  // the last steps' DMA repeats the last block into LDS that nothing reads
   settle(acc);
   __syncthreads();  // the steps' LDS becomes the waves' bands
+  static_assert(kBand<128> <= 256 * 128 && 16 * kPitch<128> * 4 <= kBand<128>, "the bands fit");
   uint8_t* const part = (wave & 2) ? (wave & 1 ? sw1 : sw0) : (wave & 1 ? sx1 : sx0);
   store_tile<true, true, ACT>(p, acc, (float*)part, m0 + wm, n0 + wn);
 }
