@@ -10,7 +10,7 @@
 //
 // What bounds it (times with the quantising pass): few rows the launch and the trip to memory (1 x 1024 x 4096: 3.3 us for
 // 4.3 MB, 96 x 4096 x 1024: 8.2); large sizes the matrix unit (8192 x 8192 x 8192: 449 us = 2.45 PFLOP/s) less the tiles' first
-// fetch and last store (14400 x 1024 x 4096 with GELU: 104 us = 1.16 PFLOP/s, four turns of 256 tiles of eight steps each).
+// fetch and last store (14400 x 1024 x 4096 with GELU: 106 us = 1.14 PFLOP/s, four turns of 256 tiles of eight steps each).
 #include <type_traits>
 
 #include "fp8.h"
