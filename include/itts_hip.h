@@ -563,7 +563,8 @@ int64_t itts_attn_cached_workspace_bytes(const ItTsKvCache* c, int B, int T, int
  * out[b][hq] = softmax(scale * q[b][hq] . K[p]) V[p] over p in [pad[b], kv_len[b]) of cache row b, hq = 0 ..
  * heads * group - 1 with K/V head hq / group; 0 where that range is empty.  pad may be NULL (0).  kv_rows
  * (optional, max_kv entries a row): key p of row b is read from cache row kv_rows[b * ld_rows + p] (the lineage table of
- * itts_attn_decode_rows); an entry outside the cache makes that row's output NaN.  kv_len outside 0 .. max_kv: NaN.
+ * itts_attn_decode_rows; ld_rows 0: one table for all rows); an entry outside the cache makes that row's output NaN.
+ * kv_len outside 0 .. max_kv: NaN.
  * max_len: the largest kv_len the caller expects (it sizes the split over keys; larger ones stay right).
  * q f32 or bf16, out bf16 or f32 (strides in elements, unit head_dim stride); out must not overlap q or the cache. */
 int itts_attn_decode_kv8(const ItTsKvCache* c, const void* q, int64_t q_sb, int64_t q_sh, int q_dtype, int B, int group,

@@ -87,7 +87,7 @@ int attend(const char* fn, AttnArgs& a, int B, int q_dtype, int out_dtype, int m
                "out must be bf16, or f32 over an e4m3 cache");
   const int64_t need = itts_attn_cached_workspace_bytes(&a.c, B, a.T, a.G, max_len, q_dtype);
   ITTS_REQUIRE(need >= 0, fn, "bad sizes (1 <= T <= 64, 1 <= group <= 4096, rows x heads x query blocks of one launch)");
-  ITTS_REQUIRE(a.kv_rows ? a.ld_rows >= a.c.max_kv : B <= a.c.rows, fn,
+  ITTS_REQUIRE(a.kv_rows ? a.ld_rows >= a.c.max_kv || a.ld_rows == 0 : B <= a.c.rows, fn,
                "more rows than the cache holds, or a short lineage table");
   ITTS_REQUIRE(a.qk_scale == a.qk_scale && a.qk_scale - a.qk_scale == 0.f, fn, "the scale must be finite");
   if (B == 0) return 0;

@@ -68,7 +68,10 @@ class _Cache:
         if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != B or t.shape[1] < self.max_kv or t.stride(1) != 1 or \
                 t.get_device() != self.index:
             raise ValueError(f"kv_rows must be int32 [{B}, >= {self.max_kv}] with unit column stride on {self.dev}")
-        return t.data_ptr(), max(t.stride(0), self.max_kv)
+        ld = t.stride(0) if B > 1 else self.max_kv
+        if 0 < ld < self.max_kv:
+            raise ValueError("rows of kv_rows must not overlap (one table expanded over all rows is taken)")
+        return t.data_ptr(), ld
 
     def _heads(self, t: torch.Tensor, shape, name: str) -> int:
         """query heads per K/V head of t [..., heads * group, head_dim]"""
@@ -182,7 +185,7 @@ class Kv8Cache(_Cache):
                out: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """Single-token attention: q [B, heads * group, head_dim] over positions pad[b] .. kv_len[b] - 1 of each row
         (this step's K/V written before); scale defaults to head_dim ** -0.5; out bf16 or f32 like q.  kv_rows
-        [B, >= max_kv] int32: the cache row that holds each position (beams).  max_len: the largest kv_len expected
+        [B, >= max_kv] int32: the cache row that holds each position (beams; one table may be expanded over the rows).  max_len: the largest kv_len expected
         (the split over keys is sized by it; default max_kv)."""
         shape = q.shape
         if len(shape) != 3:

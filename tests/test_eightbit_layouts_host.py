@@ -1,0 +1,32 @@
+"""8-bit operators without a GPU: layouts of the arguments that the calls derive pitches and offsets from."""
+import ctypes
+
+import pytest
+import torch
+
+
+def test_lineage_table_rows_are_read_where_they_are():
+    """one table expanded over the rows has row stride 0: no pitch may be made up for it"""
+    from indextts.gpt.kv8 import _Cache
+    c = object.__new__(_Cache)
+    c.rows, c.max_kv, c.index, c.dev = 4, 40, -1, torch.device("cpu")  # get_device() of a CPU tensor is -1
+    table = torch.zeros(3, 45, dtype=torch.int32)
+    assert c._lineage(table, 3) == (table.data_ptr(), 45)
+    assert c._lineage(table[:1].expand(3, -1), 3) == (table.data_ptr(), 0)
+    assert c._lineage(table[1:2, 2:], 1) == (table[1, 2:].data_ptr(), 40)
+    assert c._lineage(table[:1].expand(1, -1), 1)[1] == 40
+    with pytest.raises(ValueError):
+        c._lineage(torch.zeros(100, dtype=torch.int32).as_strided((3, 40), (20, 1)), 3)
+
+
+def test_one_lineage_table_for_all_rows():
+    from indextts import _build, _hip
+    _build.build(verbose=False)
+    lib = _hip.load()
+    c = ctypes.byref(_hip.KvCache(k=4096, v=8192, k_scale=1, v_scale=1, bs=4 * 32 * 64, hs=32 * 64, sbs=128, shs=32, rows=2,
+                                  heads=4, max_kv=32, head_dim=64, dtype=_hip.E4M3))
+
+    def decode(ld):  # no rows: nothing is launched
+        return lib.itts_attn_decode_kv8(c, 16, 256, 64, 0, 0, 1, 4, None, 4, ld, 1.0, 32, 16, 256, 64, 0, 16, None)
+
+    assert decode(0) == 0 and decode(32) == 0 and decode(31) != 0 and decode(-32) != 0
