@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "fp8.h"
+#include "fp8_rows.h"
 
 namespace {
 
@@ -325,8 +326,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void fp8_linear_tile_ke
 #pragma unroll
   for (int i = 0; i < WI; ++i) {
     const int row = 8 * (wave * WI + i) + dr;
-    const int n = (row & ~63) + 16 * (row >> 2 & 3) + 4 * (row >> 4 & 3) + (row & 3);
-    woff[i] = (uint32_t)min(n, p.N - 1 - n0) * (uint32_t)p.ldw + 16 * (ds ^ (row >> 1 & 7));
+    woff[i] = (uint32_t)itts::fetched_row(row, p.N - 1 - n0) * (uint32_t)p.ldw + 16 * (ds ^ (row >> 1 & 7));
   }
   auto issue = [&](int kb, uint8_t* X, uint8_t* W) {
 #pragma unroll
@@ -348,8 +348,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void fp8_linear_tile_ke
         const int64_t left = p.M - 1 - m0;
         src = p.xs + (m0 + (row < left ? row : left)) * p.ldxs;
       } else {
-        const int i = row - BM, n = (i & ~63) + 16 * (i >> 2 & 3) + 4 * (i >> 4 & 3) + (i & 3);
-        src = p.ws + (int64_t)min(n0 + n, p.N - 1) * p.ldws;
+        src = p.ws + (int64_t)(n0 + itts::fetched_row(row - BM, p.N - 1 - n0)) * p.ldws;
       }
       for (int d = 0; d < min(kScaleBlocks, p.KB - kb + 3) >> 2; ++d)
         ((uint32_t*)ss)[row * (kScaleBlocks / 4) + (d ^ (row >> 2 & 15))] = ((const uint32_t*)(src + kb))[d];
@@ -453,8 +452,8 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void fp8_linear_tile_ke
 // products with the fragments of later rows requested between them.  The step's one barrier stands before its last three
 // rows, when all of the step's fragments are in registers: behind it the step's LDS is free for the DMA of the step after
 // next, which has a whole step to land, and the next step's fragments are read under the last rows' products.
-// Rows of x behind M are read from the workspace's padding (their results are not stored); rows of w behind N by the
-// bounds of the buffer resource as 0.
+// Rows of x behind M are read from the workspace's padding, for rows of w behind N the last row again (their results are not
+// stored): every address lies within its buffer, none is left to the buffer resource's bounds.
 template <typename T>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const T* p, int64_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, (uint32_t)(bytes < 0xFFFFFFFFll ? bytes : 0xFFFFFFFFll), 0x00020000);
@@ -500,17 +499,17 @@ __global__ __launch_bounds__(256, 1) void fp8_linear_large_kernel(LinearArgs p) 
   const int64_t m0 = (int64_t)(lid / ntn) * 256;
   const int n0 = (lid % ntn) * 256;
 
-  // DMA instruction i of a wave fills LDS rows 64 wave + 8 i + dr; its lanes' rows and swizzle depend on i's parity alone
+  // DMA instruction i of a wave fills LDS rows 64 wave + 8 i + dr; the swizzle of its lanes' chunks depends on i's parity alone
   const int dr = lane >> 3, ds = lane & 7;
   const int ldx = (int)p.ldxq, ldw = (int)p.ldw;
   const auto xrs = buffer_of(p.xq + m0 * ldx, (int64_t)256 * ldx);
   const auto wrs = buffer_of(p.wq + (int64_t)n0 * ldw, (int64_t)(p.N - n0) * ldw);
-  uint32_t xoff[2], woff[2];
+  uint32_t xoff[2], woff[F];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int chunk = 16 * (ds ^ (4 * i + (dr >> 1)));
-    xoff[i] = dr * ldx + chunk;
-    woff[i] = (16 * (dr >> 2) + (dr & 3)) * ldw + chunk;
+  for (int i = 0; i < F; ++i) {
+    const int chunk = 16 * (ds ^ (4 * (i & 1) + (dr >> 1)));
+    if (i < 2) xoff[i] = dr * ldx + chunk;
+    woff[i] = itts::fetched_row(64 * wave + 8 * i + dr, p.N - 1 - n0) * ldw + chunk;
   }
   // x's and w's rows of a step: eight instructions each
   auto issue_x = [&](int i, int kb, uint8_t* X) {
@@ -518,8 +517,7 @@ __global__ __launch_bounds__(256, 1) void fp8_linear_large_kernel(LinearArgs p) 
                                              (64 * wave + 8 * i) * ldx + 128 * kb, 0, 0);
   };
   auto issue_w = [&](int i, int kb, uint8_t* W) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(wrs, (lds_void*)(W + 1024 * (wave * F + i)), 16, woff[i & 1],
-                                             (64 * wave + 32 * (i & 1) + 4 * (i >> 1)) * ldw + 128 * kb, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(wrs, (lds_void*)(W + 1024 * (wave * F + i)), 16, woff[i], 128 * kb, 0, 0);
   };
   // All of the tile's scale bytes, x's rows then w's in the order of its LDS rows; dword d of row i at d ^ (i / 4) % 16, so
   // that a fragment's 16 rows lie on distinct banks.  (Fetched from memory as they are needed, 16 rows far apart at a time,
@@ -528,8 +526,7 @@ __global__ __launch_bounds__(256, 1) void fp8_linear_large_kernel(LinearArgs p) 
     const int row = threadIdx.x, swz = row >> 2 & 15;
     const int64_t left = p.M - 1 - m0;
     const uint32_t* xs = (const uint32_t*)(p.xs + (m0 + (row < left ? row : left)) * p.ldxs);
-    const int n = (row & ~63) + 16 * (row >> 2 & 3) + 4 * (row >> 4 & 3) + (row & 3);
-    const uint32_t* ws = (const uint32_t*)(p.ws + (int64_t)min(n0 + n, p.N - 1) * p.ldws);
+    const uint32_t* ws = (const uint32_t*)(p.ws + (int64_t)(n0 + itts::fetched_row(row, p.N - 1 - n0)) * p.ldws);
     for (int d = 0; d < (p.KB + 3) >> 2; ++d) {
       ((uint32_t*)ss)[row * (kScaleBlocks / 4) + (d ^ swz)] = xs[d];
       ((uint32_t*)ss)[(256 + row) * (kScaleBlocks / 4) + (d ^ swz)] = ws[d];

@@ -30,3 +30,21 @@ def test_one_lineage_table_for_all_rows():
         return lib.itts_attn_decode_kv8(c, 16, 256, 64, 0, 0, 1, 4, None, 4, ld, 1.0, 32, 16, 256, 64, 0, 16, None)
 
     assert decode(0) == 0 and decode(32) == 0 and decode(31) != 0 and decode(-32) != 0
+
+
+def test_rows_fetched_for_a_tile_of_weights_lie_within_them(tmp_path):
+    """csrc/fp8_rows.h as a host program: which row of w is fetched for each of a tile's 256 (or 128) LDS rows"""
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "index-tts-dubbing_amd", "csrc")
+    src = tmp_path / "rows.cpp"
+    src.write_text('#include <cstdio>\n#include "fp8_rows.h"\nint main() { for (int last = 0; last < 256; ++last)'
+                   ' for (int i = 0; i < 256; ++i) std::printf("%d ", itts::fetched_row(i, last)); }\n')
+    subprocess.run(["g++", "-std=c++17", "-I", csrc, str(src), "-o", str(tmp_path / "rows")], check=True)
+    out = subprocess.run([str(tmp_path / "rows")], check=True, capture_output=True, text=True).stdout
+    rows = torch.tensor([int(v) for v in out.split()]).view(256, 256)
+    assert sorted(rows[255].tolist()) == list(range(256))
+    for i in range(256):  # lane r of fragment j: column 16 (r / 4) + 4 j + r % 4 of its wave's 64
+        j, r = i >> 4 & 3, i & 15
+        assert rows[255, i] == (i & 192) + 16 * (r // 4) + 4 * j + r % 4
+    assert torch.equal(rows, torch.minimum(rows[255][None], torch.arange(256)[:, None]))  # never behind the last

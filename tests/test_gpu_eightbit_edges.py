@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from test_gpu_fp8 import check as check_linear, oracle as linear_oracle
 from test_gpu_kv8 import filled, i32
 
 pytestmark = pytest.mark.gpu
@@ -22,3 +23,14 @@ def test_one_lineage_table_expanded_over_the_rows():
     assert torch.equal(c.tree(q, lens, mask, kv_rows=table), c.tree(q, lens, mask, kv_rows=table.contiguous()))
     with pytest.raises(ValueError):
         c.decode(q[:, 0], lens, kv_rows=torch.zeros(400, dtype=torch.int32, device="cuda").as_strided((B, S), (50, 1)))
+
+
+@pytest.mark.parametrize("N", [3585, 3602])
+def test_last_tile_of_few_columns(N):
+    """256 x 256 tiles whose last holds one column or 18 of w, at the end of its buffer"""
+    from indextts.utils.fp8 import Fp8Linear
+    g = torch.Generator(device="cuda").manual_seed(N)
+    x = torch.randn(3500, 1000, generator=g, device="cuda")
+    w = torch.randn(N, 1000, generator=g, device="cuda")
+    got = Fp8Linear.from_weight(w)(x, bf16_out=True)
+    check_linear(got, *linear_oracle(x, w, None, 0, None, True))
