@@ -51,11 +51,13 @@ struct AttnArgs {
   float *part, *part_ml;  // [unit][split][column][hd], [unit][split][column][maximum, sum]
 };
 
-// P is held times 2^7 relative to the column's reference, which follows the running maximum once that is more than a
-// factor 2^8 ahead: P stays within 2^15; V's codes times 2^7 relative to the largest scale: both within f16
-constexpr int kPUp = 7;
-constexpr float kLag = 8.f;
+// The column's reference follows the running maximum once that is more than a factor 2^kLag ahead.  In f16 P is held times
+// 2^kPUp relative to it, so within 2^15, and V's codes times 2^7 relative to the largest scale: both within f16.
+constexpr int kLag = 8;
+constexpr int kPUp = 15 - kLag;
 constexpr int kVUp = 7;
+// In bf16 P has f32's exponents and stays within 1: a sum of P V overflows no sooner than a sum of V.
+constexpr int kWideUp = -kLag;
 
 __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
 // low / high halves of two dwords
@@ -571,7 +573,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
       float p[8];
-      const float shift = (float)kPUp - (m[j] == -__builtin_inff() ? 0.f : m[j]);
+      const float shift = (float)(E4M3 ? kPUp : kWideUp) - (m[j] == -__builtin_inff() ? 0.f : m[j]);
 #pragma unroll
       for (int u = 0; u < 8; ++u) p[u] = __builtin_amdgcn_exp2f(fmaf(x[j][u], a.qk_scale, shift));
 #pragma unroll

@@ -2,8 +2,9 @@
 import pytest
 import torch
 
+from eightbit_util import seen_keys
 from test_gpu_fp8 import check as check_linear, oracle as linear_oracle
-from test_gpu_kv8 import filled, i32
+from test_gpu_kv8 import check_rows, filled, i32, pieces, tree_case
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +35,18 @@ def test_last_tile_of_few_columns(N):
     w = torch.randn(N, 1000, generator=g, device="cuda")
     got = Fp8Linear.from_weight(w)(x, bf16_out=True)
     check_linear(got, *linear_oracle(x, w, None, 0, None, True))
+
+
+@pytest.mark.parametrize("T,lens", [(3, [40, 0, 33]), (40, [40, 64, 7]), (2, [2000, 5, 700])])
+@pytest.mark.parametrize("q_dtype", [torch.float32, torch.bfloat16])
+def test_tree_large_finite_values_in_a_bf16_cache(T, lens, q_dtype):
+    """the largest sum of weights (relative to the largest) times |V| lies within [2^126, 2^127): finite in f32"""
+    from indextts.gpt.kv8 import Kv16Cache
+    c, k, v, q, mask = tree_case(3, T, 2, 1, 64, lens, 91, False, q_dtype)
+    see = seen_keys(3, T, k.shape[2], i32(lens), None, mask)
+    s = torch.matmul(q.double().cpu().transpose(1, 2), k.cpu().transpose(2, 3)) * 0.125
+    s = s.masked_fill(~see[:, None], -torch.inf)
+    most = torch.matmul(torch.exp(s - s.amax(-1, keepdim=True)), v.cpu().abs()).max()
+    big = (v * torch.exp2(126 - torch.floor(torch.log2(most))).cuda()).bfloat16()
+    got = Kv16Cache(c.k, big).tree(q, i32(lens), mask)
+    check_rows(got, q, k, big.double(), see, 0.125, pieces(q_dtype, torch.bfloat16, False), torch.bfloat16)
