@@ -561,7 +561,8 @@ int itts_kv8_read(const ItTsKvCache* c, const int32_t* row, const int32_t* pos, 
 int64_t itts_attn_cached_workspace_bytes(const ItTsKvCache* c, int B, int T, int group, int max_len, int q_dtype);
 /* Single-token attention over an e4m3 cache that holds this step's K/V already (itts_kv8_write):
  * out[b][hq] = softmax(scale * q[b][hq] . K[p]) V[p] over p in [pad[b], kv_len[b]) of cache row b, hq = 0 ..
- * heads * group - 1 with K/V head hq / group; 0 where that range is empty.  pad may be NULL (0).  kv_rows
+ * heads * group - 1 with K/V head hq / group; 0 where that range is empty.  Scales of V further apart than 2^12 within a row and
+ * head cost up to twice the time, not precision.  pad may be NULL (0).  kv_rows
  * (optional, max_kv entries a row): key p of row b is read from cache row kv_rows[b * ld_rows + p] (the lineage table of
  * itts_attn_decode_rows; ld_rows 0: one table for all rows); an entry outside the cache makes that row's output NaN.
  * kv_len outside 0 .. max_kv: NaN.

@@ -12,9 +12,13 @@
 // takes 16 consecutive bytes.
 //
 // Types: e4m3 K times its scale is exact in bf16 (any exponent), so q enters as bf16 and is exact when it is bf16; an f32
-// q enters as three bf16 parts (24 bits).  e4m3 V is exact in f16 relative to the largest scale of the keys seen so far
-// (2^-31 of it at the least: smaller ones round), P enters as f16 in [0, 2^15] (half step 2^-12 of a weight, below the
-// bf16 output's 2^-9) or, for f32 outputs, as two f16 parts (2^-23).  bf16 V: P as two bf16 parts (2^-17).
+// q enters as three bf16 parts (24 bits).  While the scales of a wave's V keep within a factor 2^12 of each other, e4m3 V is
+// exact in f16 relative to the largest, and P enters as f16 in [0, 2^15] (half step 2^-12 of a weight, below the bf16 output's
+// 2^-9) or, for f32 outputs, as two f16 parts (2^-23); weights below some 2^-21 of the largest keep fewer bits, those below 2^-32
+// none.  Where the scales lie further apart -- in a drafted token that other columns do not see, or in keys without
+// weight -- the wave takes its tiles once more with V as bf16, which is exact with any scale, and P as two bf16 parts (2^-17) or three
+// for f32 outputs: every finite V counts where it is seen and nowhere else.  That costs the second walk: 1.3 to 2 times the time
+// (131 keys 5.4 -> 7.0 us; 64 tokens x 4 heads over 16301 keys 110 -> 216).  bf16 V: P as two bf16 parts.
 // Maxima, sums and both products accumulate in f32.
 //
 // What bounds it, and what it takes (kernel time): few tokens over long rows run at the memory's rate (8 rows x 4 heads, up to
@@ -23,6 +27,8 @@
 // trip to memory (131 keys: 5.8 us); many columns (64 tokens x 4 heads, 16301 keys: 116 us for 27 GFLOP, 112 MB) the vector
 // instructions around the products, some 350 per 32 keys and 32 columns, half of them K's and V's conversion.
 #pragma once
+#include <type_traits>
+
 #include "fp8.h"
 
 namespace itts {
@@ -48,7 +54,7 @@ struct AttnArgs {
   // set by attend()
   bool negate, q_vec, o_vec;
   int units, qblocks, nsplit;
-  float *part, *part_ml;  // [unit][split][column][hd], [unit][split][column][maximum, sum]
+  float *part, *part_ml;  // [unit][split][column][hd], [unit][split][column][maximum, sum of weights relative to it]
 };
 
 // The column's reference follows the running maximum once that is more than a factor 2^kLag ahead.  In f16 P is held times
@@ -58,6 +64,9 @@ constexpr int kPUp = 15 - kLag;
 constexpr int kVUp = 7;
 // In bf16 P has f32's exponents and stays within 1: a sum of P V overflows no sooner than a sum of V.
 constexpr int kWideUp = -kLag;
+// Scales of V within a factor 2^kSpread of each other go through f16: V is exact there up to 2^22, and what f16 loses of a
+// weight (below 2^-32 of the largest) counts for little whatever its V.
+constexpr int kSpread = 12;
 
 __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
 // low / high halves of two dwords
@@ -253,12 +262,16 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
       }
     }
   };
-  int base = begin + 32 * wave;
-  if (base <= last) {
-    load_rows(base);
-    load(base);
-    if (base + 32 * kWaves <= last) load_rows(base + 32 * kWaves);
-  }
+  int base;
+  auto load_first = [&] {
+    base = begin + 32 * wave;
+    if (base <= last) {
+      load_rows(base);
+      load(base);
+      if (base + 32 * kWaves <= last) load_rows(base + 32 * kWaves);
+    }
+  };
+  load_first();
 
   // this lane's columns, their masks and Q
   int col[NQ], tok[NQ];
@@ -322,20 +335,27 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[j][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  int vref = 0;      // e4m3: V is held relative to 2^(vref - 127)
-  uint32_t odd = 0;  // non-zero: V held a NaN or infinity at a drafted token
+  int vref = 0;          // e4m3: V is held relative to 2^(vref - 127)
+  uint32_t low = ~0u;    // smallest scale that this lane has met, as f32 bits (less one at most)
+  uint32_t odd = 0;      // non-zero: V held a NaN or infinity at a drafted token
 
-  // V^T operands [16-dim tile][8 keys]; dim tile d holds the lane's dims (hd / 16) r + d
-  auto v_frags = [&](const uint32_t (&v)[8][KW], const float (&sc)[8], u32x4_t (&vf)[DT]) {
+  // V^T operands [16-dim tile][8 keys]; dim tile d holds the lane's dims (hd / 16) r + d.  f16: e4m3 V as f16, otherwise bf16
+  auto v_frags = [&](auto f16, const uint32_t (&v)[8][KW], const float (&sc)[8], u32x4_t (&vf)[DT]) {
+    auto two = [&](uint32_t w, float s, auto up) {
+      if constexpr (decltype(f16)::value)
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, decltype(up)::value));
+      else
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, decltype(up)::value));
+    };
+    constexpr std::false_type lower{};
+    constexpr std::true_type upper{};
 #pragma unroll
     for (int i = 0; i < KW; ++i) {
 #pragma unroll
       for (int u = 0; u < 8; u += 2) {
         if constexpr (E4M3) {
-          const uint32_t a0 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[u][i], sc[u], false));
-          const uint32_t a1 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[u][i], sc[u], true));
-          const uint32_t b0 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[u + 1][i], sc[u + 1], false));
-          const uint32_t b1 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[u + 1][i], sc[u + 1], true));
+          const uint32_t a0 = two(v[u][i], sc[u], lower), a1 = two(v[u][i], sc[u], upper);
+          const uint32_t b0 = two(v[u + 1][i], sc[u + 1], lower), b1 = two(v[u + 1][i], sc[u + 1], upper);
           vf[4 * i][u / 2] = lo16(a0, b0);
           vf[4 * i + 1][u / 2] = hi16(a0, b0);
           vf[4 * i + 2][u / 2] = lo16(a1, b1);
@@ -347,14 +367,12 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
       }
     }
   };
-  auto pv = [&](u32x4_t vf, u32x4_t pf, f32x4_t acc) -> f32x4_t {
-    if constexpr (E4M3)
+  auto pv = [&](auto f16, u32x4_t vf, u32x4_t pf, f32x4_t acc) -> f32x4_t {
+    if constexpr (decltype(f16)::value)
       return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, vf), __builtin_bit_cast(f16x8_t, pf), acc, 0, 0, 0);
     else
       return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, vf), __builtin_bit_cast(bf16x8_t, pf), acc, 0, 0, 0);
   };
-  constexpr uint32_t kOne = E4M3 ? 0x3C00u : 0x3F80u;
-  const u32x4_t ones = u32x4_t{kOne * 0x10001u, kOne * 0x10001u, kOne * 0x10001u, kOne * 0x10001u};
 
   // Which of a tile's 32 keys are seen, as bits: all columns' prefix, and a column's drafted tokens
   auto below = [](int i) -> uint32_t { return i <= 0 ? 0u : i >= 32 ? ~0u : (1u << i) - 1; };  // bits 0 .. i - 1
@@ -368,6 +386,8 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
   // A drafted token's V that is not finite reaches only the columns that see it.  Such values enter the products as 0;
   // here a product of (1 where V is the special value) and (1 where the column sees the key) counts them.
   auto not_finite = [&](int tile) {
+    constexpr std::bool_constant<E4M3> f16{};
+    constexpr uint32_t kOne = E4M3 ? 0x3C00u : 0x3F80u;
     const uint32_t drafted = mine(below(hi - tile) & ~below(len - tile));
     uint32_t w8[8][KW];
 #pragma unroll
@@ -405,7 +425,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
         }
       }
       u32x4_t nf[DT];
-      v_frags(ind, one, nf);
+      v_frags(f16, ind, one, nf);
       const float what = kind == 0 ? __builtin_nanf("") : kind == 1 ? __builtin_inff() : -__builtin_inff();
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
@@ -415,7 +435,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
         for (int e = 0; e < 4; ++e) pf[e] = (vis >> (2 * e) & 1) * kOne | (vis >> (2 * e + 1) & 1) * (kOne << 16);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          const f32x4_t count = pv(nf[d], pf, f32x4_t{0.f, 0.f, 0.f, 0.f});
+          const f32x4_t count = pv(f16, nf[d], pf, f32x4_t{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (count[i] > 0.f) o[j][d][i] += what;
@@ -424,199 +444,255 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
     }
   };
 
-  for (; base < end; base += 32 * kWaves) {
-    const int tile = base;
-    // an edge tile holds keys that some column may not see (before the padding's end, drafted, behind the row's end)
-    const bool edge = tile < first || tile + 32 > len;
-    uint32_t some = 0xFF;  // which of the lane's eight keys some column may see
-    if (edge) {
-      const uint32_t drafted = mine(below(hi - tile) & ~below(len - tile));
-      some = mine(prefix_bits(tile)) | drafted;
+  // The loop over the tiles.  wide: V as bf16, exact with any scale, and P in one more part of 8 bits each instead of 11.
+  auto walk = [&](auto wide) {
+    constexpr bool WIDE = decltype(wide)::value, F16 = E4M3 && !WIDE;
+    constexpr std::bool_constant<F16> f16{};
+    constexpr int PP = PN + (WIDE ? 1 : 0);
+    constexpr uint32_t kOnes = (F16 ? 0x3C00u : 0x3F80u) * 0x10001u;
+    const u32x4_t ones = u32x4_t{kOnes, kOnes, kOnes, kOnes};
+    for (; base < end; base += 32 * kWaves) {
+      const int tile = base;
+      // an edge tile holds keys that some column may not see (before the padding's end, drafted, behind the row's end)
+      const bool edge = tile < first || tile + 32 > len;
+      uint32_t some = 0xFF;  // which of the lane's eight keys some column may see
+      if (edge) {
+        const uint32_t drafted = mine(below(hi - tile) & ~below(len - tile));
+        some = mine(prefix_bits(tile)) | drafted;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
+        for (int u = 0; u < 8; ++u) {
 #pragma unroll
-        for (int i = 0; i < KW; ++i) {
-          const uint32_t w = some >> u & 1 ? tv[u][i] : 0u;
-          uint32_t bits;  // a drafted token's values that are not finite
-          if constexpr (E4M3) bits = (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
-          else bits = (((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u) >> 15;
-          bits *= (drafted >> u & 1) * (E4M3 ? 0xFFu : 0xFFFFu);
-          odd |= bits;
-          tv[u][i] = w & ~bits;
+          for (int i = 0; i < KW; ++i) {
+            const uint32_t w = some >> u & 1 ? tv[u][i] : 0u;
+            uint32_t bits;  // a drafted token's values that are not finite
+            if constexpr (E4M3) bits = (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
+            else bits = (((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u) >> 15;
+            bits *= (drafted >> u & 1) * (E4M3 ? 0xFFu : 0xFFFFu);
+            odd |= bits;
+            tv[u][i] = w & ~bits;
+          }
         }
       }
-    }
-    float sv[8];
-    float rescale = 1.f;
-    if constexpr (E4M3) {
-      int vs[8];  // the scales as f32 bits, which order like them
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const uint32_t w = tvs[u >> 2];
-        vs[u] = ((u & 3) == 3 ? w >> 1 : w << (23 - 8 * (u & 3))) & 0x7F800000u;
-      }
-      if (edge) {  // what nothing is seen of has no part in the reference; its V is 0
-#pragma unroll
-        for (int u = 0; u < 8; ++u) vs[u] = some >> u & 1 ? vs[u] : 0;
-      }
-      int top = max(max(max(vs[0], vs[1]), max(vs[2], vs[3])), max(max(vs[4], vs[5]), max(vs[6], vs[7])));
-      top = __builtin_amdgcn_readfirstlane(max_rows(top)) >> 23;  // 16 lanes each hold the same eight bytes
-      if (top > vref) {
-        rescale = vref == 0 ? 0.f : __builtin_amdgcn_exp2f((float)(vref - top));
-        vref = top;
-      }
-#pragma unroll
-      for (int u = 0; u < 8; ++u) sv[u] = __builtin_ldexpf(__uint_as_float(vs[u]), 127 + kVUp - vref);
-    }
-    u32x4_t vf[DT], kf[2][KS];
-    v_frags(tv, sv, vf);
-#pragma unroll
-    for (int f = 0; f < 2; ++f) {
+      float sv[8];
+      float rescale = 1.f;
       if constexpr (E4M3) {
-        const float sc = itts::e4m3_scale(tks[f]);
+        int vs[8];  // the scales as f32 bits, which order like them
 #pragma unroll
-        for (int i = 0; i < KW; ++i)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            kf[f][2 * i + (w >> 1)][2 * (w & 1)] =
-                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(tk[f][i][w], sc, false));
-            kf[f][2 * i + (w >> 1)][2 * (w & 1) + 1] =
-                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(tk[f][i][w], sc, true));
-          }
-      } else {
-#pragma unroll
-        for (int s = 0; s < KS; ++s) kf[f][s] = tk[f][s];
-      }
-    }
-    const uint32_t bad = tbad;
-    const bool any_bad = LINEAGE && __any(bad != 0);
-    // the tile is in its operands: the next one is requested into the same registers
-    if (tile + 32 * kWaves < end) {
-      load(tile + 32 * kWaves);
-      if (LINEAGE && tile + 64 * kWaves < end) load_rows(tile + 64 * kWaves);
-    }
-    // the columns' scores and their maxima (a.qk_scale > 0); all columns go through each stage together, so that
-    // one's products cover another's latencies
-    float x[NQ][8], top[NQ];
-    bool grow = rescale != 1.f;
-    auto scores = [&](const u32x4_t (&low)[2][KS]) {  // low: what the lower parts of q meet
-#pragma unroll
-      for (int j = 0; j < NQ; ++j) {
-        f32x4_t s[2];
-#pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          s[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int e = 0; e < KS; ++e)
-#pragma unroll
-            for (int q = QN - 1; q >= 0; --q)
-              s[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, q ? low[f][e] : kf[f][e]),
-                                                             __builtin_bit_cast(bf16x8_t, qf[j][e][q]), s[f], 0, 0, 0);
+        for (int u = 0; u < 8; ++u) {
+          const uint32_t w = tvs[u >> 2];
+          vs[u] = ((u & 3) == 3 ? w >> 1 : w << (23 - 8 * (u & 3))) & 0x7F800000u;
         }
+        if (edge) {  // what nothing is seen of has no part in the reference; its V is 0
 #pragma unroll
-        for (int u = 0; u < 8; ++u) x[j][u] = s[u >> 2][u & 3];
+          for (int u = 0; u < 8; ++u) vs[u] = some >> u & 1 ? vs[u] : 0;
+#pragma unroll
+          for (int u = 0; u < 8; ++u) low = min(low, (uint32_t)vs[u] - 1);  // 0, an unseen key's, becomes the largest
+        } else {
+#pragma unroll
+          for (int u = 0; u < 8; ++u) low = min(low, (uint32_t)vs[u]);
+        }
+        if constexpr (WIDE) {
+#pragma unroll
+          for (int u = 0; u < 8; ++u) sv[u] = __uint_as_float(vs[u]);
+        } else {
+          int top = max(max(max(vs[0], vs[1]), max(vs[2], vs[3])), max(max(vs[4], vs[5]), max(vs[6], vs[7])));
+          top = __builtin_amdgcn_readfirstlane(max_rows(top)) >> 23;  // 16 lanes each hold the same eight bytes
+          if (top > vref) {
+            rescale = vref == 0 ? 0.f : __builtin_amdgcn_exp2f((float)(vref - top));
+            vref = top;
+          }
+#pragma unroll
+          for (int u = 0; u < 8; ++u) sv[u] = __builtin_ldexpf(__uint_as_float(vs[u]), 127 + kVUp - vref);
+        }
       }
-    };
-    scores(kf);
-    if constexpr (!E4M3 && QN > 1) {  // an infinite K times a lower part of 0 is NaN: once more without such products
-      bool nan = false;
+      u32x4_t vf[DT], kf[2][KS];
+      v_frags(f16, tv, sv, vf);
 #pragma unroll
-      for (int j = 0; j < NQ; ++j)
+      for (int f = 0; f < 2; ++f) {
+        if constexpr (E4M3) {
+          const float sc = itts::e4m3_scale(tks[f]);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) nan |= x[j][u] != x[j][u];
-      if (__any(nan)) {
-        u32x4_t low[2][KS];
+          for (int i = 0; i < KW; ++i)
 #pragma unroll
-        for (int f = 0; f < 2; ++f)
-#pragma unroll
-          for (int e = 0; e < KS; ++e)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t w = kf[f][e][i];
-              low[f][e][i] = w & ~(((((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u) >> 15) * 0xFFFFu);
+            for (int w = 0; w < 4; ++w) {
+              kf[f][2 * i + (w >> 1)][2 * (w & 1)] =
+                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(tk[f][i][w], sc, false));
+              kf[f][2 * i + (w >> 1)][2 * (w & 1) + 1] =
+                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(tk[f][i][w], sc, true));
             }
-        scores(low);
-      }
-    }
-    if (any_bad) {
+        } else {
 #pragma unroll
-      for (int j = 0; j < NQ; ++j)
-#pragma unroll
-        for (int u = 0; u < 8; ++u) x[j][u] = bad >> u & 1 ? __builtin_nanf("") : x[j][u];
-    }
-    if (edge) {
-#pragma unroll
-      for (int j = 0; j < NQ; ++j) {
-        const uint32_t vis = mine(prefix_bits(tile) | drafted_bits(tile, msk[j]));
-#pragma unroll
-        for (int u = 0; u < 8; ++u) x[j][u] = vis >> u & 1 ? x[j][u] : -__builtin_inff();
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < NQ; ++j) {
-      top[j] = max_rows(max2(max2(max2(x[j][0], x[j][1]), max2(x[j][2], x[j][3])),
-                             max2(max2(x[j][4], x[j][5]), max2(x[j][6], x[j][7]))) * a.qk_scale);
-      grow |= top[j] > m[j] + kLag;
-    }
-    if (__any(grow)) {
-#pragma unroll
-      for (int j = 0; j < NQ; ++j) {
-        const float next = fmaxf(m[j], top[j]);
-        const float f = next == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m[j] - next);
-        m[j] = next;
-        l[j] = l[j] * f;
-        const float fo = f * rescale;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[j][d] = o[j][d] * fo;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < NQ; ++j) {
-      float p[8];
-      const float shift = (float)(E4M3 ? kPUp : kWideUp) - (m[j] == -__builtin_inff() ? 0.f : m[j]);
-#pragma unroll
-      for (int u = 0; u < 8; ++u) p[u] = __builtin_amdgcn_exp2f(fmaf(x[j][u], a.qk_scale, shift));
-#pragma unroll
-      for (int q = 0; q < PN; ++q) {
-        u32x4_t pf;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (E4M3) {
-            const f16x2_t w = {(_Float16)p[2 * e], (_Float16)p[2 * e + 1]};
-            pf[e] = __builtin_bit_cast(uint32_t, w);
-            if (q + 1 < PN) p[2 * e] -= (float)w[0], p[2 * e + 1] -= (float)w[1];
-          } else {
-            const uint32_t w = pack2bf(p[2 * e], p[2 * e + 1]);
-            pf[e] = w;
-            if (q + 1 < PN) p[2 * e] -= __uint_as_float(w << 16), p[2 * e + 1] -= __uint_as_float(w & 0xFFFF0000u);
-          }
+          for (int s = 0; s < KS; ++s) kf[f][s] = tk[f][s];
         }
-        l[j] = pv(ones, pf, l[j]);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[j][d] = pv(vf[d], pf, o[j][d]);
       }
+      const uint32_t bad = tbad;
+      const bool any_bad = LINEAGE && __any(bad != 0);
+      // the tile is in its operands: the next one is requested into the same registers
+      if (tile + 32 * kWaves < end) {
+        load(tile + 32 * kWaves);
+        if (LINEAGE && tile + 64 * kWaves < end) load_rows(tile + 64 * kWaves);
+      }
+      // the columns' scores and their maxima (a.qk_scale > 0); all columns go through each stage together, so that
+      // one's products cover another's latencies
+      float x[NQ][8], top[NQ];
+      bool grow = rescale != 1.f;
+      auto scores = [&](const u32x4_t (&low)[2][KS]) {  // low: what the lower parts of q meet
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+          f32x4_t s[2];
+#pragma unroll
+          for (int f = 0; f < 2; ++f) {
+            s[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < KS; ++e)
+#pragma unroll
+              for (int q = QN - 1; q >= 0; --q)
+                s[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, q ? low[f][e] : kf[f][e]),
+                                                               __builtin_bit_cast(bf16x8_t, qf[j][e][q]), s[f], 0, 0, 0);
+          }
+#pragma unroll
+          for (int u = 0; u < 8; ++u) x[j][u] = s[u >> 2][u & 3];
+        }
+      };
+      scores(kf);
+      if constexpr (!E4M3 && QN > 1) {  // an infinite K times a lower part of 0 is NaN: once more without such products
+        bool nan = false;
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+          for (int u = 0; u < 8; ++u) nan |= x[j][u] != x[j][u];
+        if (__any(nan)) {
+          u32x4_t low[2][KS];
+#pragma unroll
+          for (int f = 0; f < 2; ++f)
+#pragma unroll
+            for (int e = 0; e < KS; ++e)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t w = kf[f][e][i];
+                low[f][e][i] = w & ~(((((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u) >> 15) * 0xFFFFu);
+              }
+          scores(low);
+        }
+      }
+      if (any_bad) {
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+          for (int u = 0; u < 8; ++u) x[j][u] = bad >> u & 1 ? __builtin_nanf("") : x[j][u];
+      }
+      if (edge) {
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+          const uint32_t vis = mine(prefix_bits(tile) | drafted_bits(tile, msk[j]));
+#pragma unroll
+          for (int u = 0; u < 8; ++u) x[j][u] = vis >> u & 1 ? x[j][u] : -__builtin_inff();
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        top[j] = max_rows(max2(max2(max2(x[j][0], x[j][1]), max2(x[j][2], x[j][3])),
+                               max2(max2(x[j][4], x[j][5]), max2(x[j][6], x[j][7]))) * a.qk_scale);
+        grow |= top[j] > m[j] + kLag;
+      }
+      if (__any(grow)) {
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+          const float next = fmaxf(m[j], top[j]);
+          const float f = next == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m[j] - next);
+          m[j] = next;
+          l[j] = l[j] * f;
+          const float fo = f * rescale;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[j][d] = o[j][d] * fo;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        float p[8];
+        const float shift = (float)(F16 ? kPUp : kWideUp) - (m[j] == -__builtin_inff() ? 0.f : m[j]);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) p[u] = __builtin_amdgcn_exp2f(fmaf(x[j][u], a.qk_scale, shift));
+#pragma unroll
+        for (int q = 0; q < PP; ++q) {
+          u32x4_t pf;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (F16) {
+              const f16x2_t w = {(_Float16)p[2 * e], (_Float16)p[2 * e + 1]};
+              pf[e] = __builtin_bit_cast(uint32_t, w);
+              if (q + 1 < PP) p[2 * e] -= (float)w[0], p[2 * e + 1] -= (float)w[1];
+            } else {
+              const uint32_t w = pack2bf(p[2 * e], p[2 * e + 1]);
+              pf[e] = w;
+              if (q + 1 < PP) p[2 * e] -= __uint_as_float(w << 16), p[2 * e + 1] -= __uint_as_float(w & 0xFFFF0000u);
+            }
+          }
+          l[j] = pv(f16, ones, pf, l[j]);
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[j][d] = pv(f16, vf[d], pf, o[j][d]);
+        }
+      }
+    }  };
+  bool absolute = !E4M3;  // o holds sums of P V as they are
+  walk(std::false_type{});
+  if constexpr (E4M3) {
+    if (__builtin_expect(__any((int)min(low, kInfBits) < (vref - kSpread) * (1 << 23) - 1), 0)) {  // V's scales turned out too far apart: all tiles once more
+      absolute = true;
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        m[j] = -__builtin_inff();
+        l[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[j][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      }
+      load_first();
+      walk(std::true_type{});
     }
   }
-  if (__any(odd != 0)) {  // the drafted tokens' tiles of this wave once more
+  if (__builtin_expect(__any(odd != 0), 0)) {  // the drafted tokens' tiles of this wave once more
     for (int tile = begin + 32 * wave; tile < end; tile += 32 * kWaves)
       if (tile + 32 > len) not_finite(tile);
   }
 
   // ---- the waves' parts: common maximum and V reference, then O and the sums added in wave order ----
+  // The common V reference is the largest.  Where a wave has none, or the waves' lie so far apart that f32 would lose the least
+  // beside it, O is brought to the sums of P V that it stands for, with P in bf16's scale.
   constexpr int LDC = HD + 4;
   __shared__ float so[kWaves][COLS][LDC];
   __shared__ float sm[kWaves][COLS], sl[kWaves][COLS];
   __shared__ int sr[kWaves];
-  if (lane == 0) sr[wave] = vref;
+  if (lane == 0) sr[wave] = absolute ? -1 : vref;
   if (c == 0) {
 #pragma unroll
     for (int j = 0; j < NQ; ++j) sm[wave][16 * j + r] = m[j];
   }
   __syncthreads();
-  int top_ref = 0;
+  int up = 0, p_up = kWideUp;  // O holds its values times 2^-up, and P's scale is 2^p_up
+  float rel = 1.f;             // what this wave's O is brought to the common reference by
   if constexpr (E4M3) {
+    int top_ref = 0, low_ref = 255;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) top_ref = max(top_ref, sr[w]);
+    for (int w = 0; w < kWaves; ++w) {
+      top_ref = max(top_ref, sr[w]);
+      low_ref = min(low_ref, sr[w] == 0 ? 255 : sr[w]);
+    }
+    if (__builtin_expect(low_ref < top_ref - 64 || low_ref < 0, 0)) {
+      if (!absolute) {
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+          l[j][0] = __builtin_ldexpf(l[j][0], kWideUp - kPUp);
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[j][d][i] = __builtin_ldexpf(o[j][d][i], vref - 127 - kVUp + kWideUp - kPUp);
+        }
+      }
+    } else {
+      up = top_ref - 127 - kVUp;
+      p_up = kPUp;
+      rel = __builtin_amdgcn_exp2f((float)(vref - top_ref));  // 0 for a wave without keys
+    }
   }
 #pragma unroll
   for (int j = 0; j < NQ; ++j) {
@@ -625,7 +701,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, sm[w][16 * j + r]);
     const float fl = top == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(m[j] - top);
-    const float fo = E4M3 ? fl * __builtin_amdgcn_exp2f((float)(vref - top_ref)) : fl;
+    const float fo = fl * rel;
     if (c == 0) sl[wave][16 * j + r] = l[j][0] * fl;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -635,7 +711,9 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
             f32x4_t{o[j][d][i] * fo, o[j][d + 1][i] * fo, o[j][d + 2][i] * fo, o[j][d + 3][i] * fo};
   }
   __syncthreads();
-  const float vscale = E4M3 ? __builtin_amdgcn_exp2f((float)(top_ref - 127 - kVUp)) : 1.f;
+  auto times = [](f32x4_t v, int e) -> f32x4_t {
+    return f32x4_t{__builtin_ldexpf(v[0], e), __builtin_ldexpf(v[1], e), __builtin_ldexpf(v[2], e), __builtin_ldexpf(v[3], e)};
+  };
   const int cols = min(COLS, C - qb * COLS);
   for (int i = threadIdx.x; i < cols * (HD / 4); i += 64 * kWaves) {
     const int cl = i / (HD / 4), d = 4 * (i - cl * (HD / 4));
@@ -648,20 +726,21 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
     }
     const int cg = qb * COLS + cl;
     if (a.nsplit > 1) {
+      // the split's own result, which is no larger than V, and its weight among the splits
       const int64_t at = ((int64_t)unit * a.nsplit + split) * C + cg;
-      *reinterpret_cast<f32x4_t*>(a.part + at * HD + d) = acc * vscale;
+      *reinterpret_cast<f32x4_t*>(a.part + at * HD + d) = times(acc * (sum == 0.f ? 1.f : 1.f / sum), up);
       if (d == 0) {
         float top = -__builtin_inff();
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) top = fmaxf(top, sm[w][cl]);
         a.part_ml[2 * at] = top;
-        a.part_ml[2 * at + 1] = sum;
+        a.part_ml[2 * at + 1] = __builtin_ldexpf(sum, -p_up);
       }
     } else {
       const int t = cg / G;
       if (!refuse && t >= nt) continue;
-      const float inv = refuse ? __builtin_nanf("") : vscale * inverse_sum(a, sum, b, t, len, n);
-      store4(a, (int64_t)b * a.o_sb + t * a.o_st + (int64_t)(h * G + cg - t * G) * a.o_sh + d, acc * inv);
+      const float inv = refuse ? __builtin_nanf("") : inverse_sum(a, sum, b, t, len, n);
+      store4(a, (int64_t)b * a.o_sb + t * a.o_st + (int64_t)(h * G + cg - t * G) * a.o_sh + d, times(acc * inv, up));
     }
   }
 }

@@ -9,7 +9,7 @@ namespace {
 
 using namespace itts::attn;
 
-// the splits' parts of one column: common maximum, O and the sums added in split order; one wave per column
+// the splits' results of one column, each times its share of the weights, added in split order; one wave per column
 template <int HD>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   const int C = a.T * a.G;
@@ -42,29 +42,23 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   top = wave_max(top);
   const float ref = top == -__builtin_inff() ? 0.f : top;
   float sum = 0.f;
+  for (int s = lane; s < a.nsplit; s += 64)
+    sum += __builtin_amdgcn_exp2f(a.part_ml[2 * at(s)] - ref) * a.part_ml[2 * at(s) + 1];
+  sum = wave_sum(sum);
+  const float inv = refuse ? __builtin_nanf("") : inverse_sum(a, sum, b, t, len, n);
   f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < EARLY; ++i) {
-    if (g + P * i < a.nsplit) {
-      const float f = __builtin_amdgcn_exp2f(em[i] - ref);
-      sum += f * el[i];
-      acc = acc + early[i] * f;
-    }
-  }
-  for (int s = g + P * EARLY; s < a.nsplit; s += P) {
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at(s)] - ref);
-    sum += f * a.part_ml[2 * at(s) + 1];
-    acc = acc + *reinterpret_cast<const f32x4_t*>(a.part + at(s) * HD + d) * f;
-  }
+  for (int i = 0; i < EARLY; ++i)
+    if (g + P * i < a.nsplit) acc = acc + early[i] * (__builtin_amdgcn_exp2f(em[i] - ref) * el[i] * inv);
+  for (int s = g + P * EARLY; s < a.nsplit; s += P)
+    acc = acc + *reinterpret_cast<const f32x4_t*>(a.part + at(s) * HD + d) *
+                    (__builtin_amdgcn_exp2f(a.part_ml[2 * at(s)] - ref) * a.part_ml[2 * at(s) + 1] * inv);
 #pragma unroll
-  for (int o = L; o < 64; o <<= 1) {
-    sum += __shfl_xor(sum, o, 64);
+  for (int o = L; o < 64; o <<= 1)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], o, 64);
-  }
   if (g != 0) return;
-  const float inv = refuse ? __builtin_nanf("") : inverse_sum(a, sum, b, t, len, n);
-  store4(a, (int64_t)b * a.o_sb + t * a.o_st + (int64_t)(h * a.G + cg - t * a.G) * a.o_sh + d, acc * inv);
+  store4(a, (int64_t)b * a.o_sb + t * a.o_st + (int64_t)(h * a.G + cg - t * a.G) * a.o_sh + d, acc);
 }
 
 int query_blocks(bool e4m3, int cols, bool q_f32, int hd) {

@@ -185,8 +185,8 @@ class Kv8Cache(_Cache):
                out: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """Single-token attention: q [B, heads * group, head_dim] over positions pad[b] .. kv_len[b] - 1 of each row
         (this step's K/V written before); scale defaults to head_dim ** -0.5; out bf16 or f32 like q.  kv_rows
-        [B, >= max_kv] int32: the cache row that holds each position (beams; one table may be expanded over the rows).  max_len: the largest kv_len expected
-        (the split over keys is sized by it; default max_kv)."""
+        [B, >= max_kv] int32: the cache row that holds each position (beams; one table may be expanded over the rows).
+        max_len: the largest kv_len expected (the split over keys is sized by it; default max_kv)."""
         shape = q.shape
         if len(shape) != 3:
             raise ValueError(f"q must be [B, heads, head_dim], got {tuple(shape)}")

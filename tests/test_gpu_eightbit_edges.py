@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from eightbit_util import seen_keys
+from eightbit_util import attend64, attn_tol, codes64, seen_keys
 from test_gpu_fp8 import check as check_linear, oracle as linear_oracle
 from test_gpu_kv8 import check_rows, filled, i32, pieces, tree_case
 
@@ -50,3 +50,114 @@ def test_tree_large_finite_values_in_a_bf16_cache(T, lens, q_dtype):
     big = (v * torch.exp2(126 - torch.floor(torch.log2(most))).cuda()).bfloat16()
     got = Kv16Cache(c.k, big).tree(q, i32(lens), mask)
     check_rows(got, q, k, big.double(), see, 0.125, pieces(q_dtype, torch.bfloat16, False), torch.bfloat16)
+
+
+# ---- scales of V far apart in an 8-bit cache: every value within f32's range counts where it is seen, and only there ----
+
+OUT = [(torch.bfloat16, torch.bfloat16), (torch.float32, torch.bfloat16), (torch.float32, torch.float32), (torch.bfloat16, torch.float32)]
+
+
+def raised(c, places, by):
+    """c's V times 2^by at places (an index of [rows, heads, max_kv]); the values it then stands for"""
+    c.v_scale[places] += by
+    return codes64(c.v, c.v_scale)
+
+
+def identity(B, S):
+    return torch.arange(B, device="cuda", dtype=torch.int32)[:, None].repeat(1, S)
+
+
+@pytest.mark.parametrize("q_dtype,out_dtype", OUT)
+@pytest.mark.parametrize("hd,heads,group", [(64, 2, 1), (128, 1, 3)])
+@pytest.mark.parametrize("T", [4, 20])
+@pytest.mark.parametrize("by", [25, 40, 100])
+def test_a_drafted_token_with_a_large_v_reaches_only_its_own(q_dtype, out_dtype, hd, heads, group, T, by):
+    lens = [0, 30, 64, 1500]
+    c, k, v, q, mask = tree_case(4, T, heads, group, hd, lens, by, True, q_dtype)
+    for b, n in enumerate(lens):
+        v = raised(c, (b, slice(None), n + 2), by)
+    see = seen_keys(4, T, k.shape[2], i32(lens), None, mask)
+    for rows in (None, identity(4, k.shape[2])):
+        got = c.tree(q, i32(lens), mask, kv_rows=rows, dtype=out_dtype)
+        check_rows(got, q, k, v, see, hd ** -0.5, pieces(q_dtype, out_dtype), out_dtype)
+
+
+@pytest.mark.parametrize("q_dtype,out_dtype", OUT)
+@pytest.mark.parametrize("by", [20, 60, 80, 110])
+def test_waves_whose_scales_are_far_apart(q_dtype, out_dtype, by):
+    """two drafted tokens in a tile of their own, both with a large V, of which the second sees neither"""
+    lens = [32, 64, 96, 2048]
+    c, k, v, q, _ = tree_case(4, 2, 2, 2, 64, lens, by, True, q_dtype)
+    mask = torch.tensor([1, 0], device="cuda")
+    for b, n in enumerate(lens):
+        v = raised(c, (b, slice(None), slice(n, n + 2)), by)
+    got = c.tree(q, i32(lens), mask, dtype=out_dtype)
+    check_rows(got, q, k, v, seen_keys(4, 2, k.shape[2], i32(lens), None, mask), 0.125, pieces(q_dtype, out_dtype), out_dtype)
+
+
+@pytest.mark.parametrize("q_dtype,out_dtype", OUT)
+@pytest.mark.parametrize("hd,heads,group", [(64, 2, 1), (128, 1, 20)])
+def test_keys_whose_scales_are_far_apart(q_dtype, out_dtype, hd, heads, group):
+    """large V with next to no weight beside small V with all of it, and V of every scale"""
+    lens = i32([1, 50, 300, 1999])
+    c, k, v = filled(4, heads, 2000, hd, seed=5)
+    g = torch.Generator().manual_seed(6)
+    q = (torch.randn(4, heads * group, hd, generator=g) * 2).to(q_dtype).cuda()
+    see = seen_keys(4, 1, 2000, lens)
+    c.k_scale[:, :, 7] += 3  # wide scores: some keys have weights of 2^-40 and less
+    c.k_scale[:, :, 100::9] += 3
+    k = codes64(c.k, c.k_scale)
+    v = raised(c, (slice(None), slice(None), slice(7, None, 31)), 30)
+    for _ in range(2):
+        got = c.decode(q, lens, dtype=out_dtype)
+        check_rows(got[:, None], q[:, None], k, v, see, hd ** -0.5, pieces(q_dtype, out_dtype), out_dtype)
+        c.v_scale.copy_(torch.randint(30, 230, c.v_scale.shape, generator=g, dtype=torch.uint8))
+        v = codes64(c.v, c.v_scale)
+
+
+@pytest.mark.parametrize("q_dtype,out_dtype", OUT)
+def test_loud_dims(q_dtype, out_dtype):
+    """some keys hold one dim 2^30 above the others (whose codes are 0): the other keys' values still make the other dims"""
+    from indextts.gpt.kv8 import Kv8Cache
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn(2, 100, 2, 64, generator=g)
+    y = x.clone()
+    y[:, 5::20, :, 9] = 2.0 ** 30
+    c = Kv8Cache.empty(2, 2, 100, 64)
+    row, pos = torch.arange(2).repeat_interleave(100).int().cuda(), torch.arange(100).repeat(2).int().cuda()
+    c.write(x.view(-1, 2, 64).cuda(), y.view(-1, 2, 64).cuda(), row, pos)
+    q = torch.randn(2, 2, 64, generator=g).to(q_dtype).cuda()
+    k, v = codes64(c.k, c.k_scale), codes64(c.v, c.v_scale)
+    got = c.decode(q, i32([100, 61]), dtype=out_dtype)
+    check_rows(got[:, None], q[:, None], k, v, seen_keys(2, 1, 100, i32([100, 61])), 0.125, pieces(q_dtype, out_dtype), out_dtype)
+
+
+@pytest.mark.parametrize("q_dtype,out_dtype", OUT)
+@pytest.mark.parametrize("by", [-100, -60, 60, 105])
+def test_v_at_the_ends_of_the_range(q_dtype, out_dtype, by):
+    """all V times 2^by: the results times 2^by"""
+    lens = i32([3, 40, 1400])
+    c, k, v = filled(3, 2, 1400, 64, seed=12)
+    q = torch.randn(3, 4, 64, generator=torch.Generator().manual_seed(13)).to(q_dtype).cuda()
+    v = raised(c, (slice(None),) * 3, by % 256)
+    got = c.decode(q, lens, dtype=out_dtype).double() * 2.0 ** -by
+    ref, mag, top = attend64(q[:, None].double(), k, v * 2.0 ** -by, seen_keys(3, 1, 1400, lens), 0.125)
+    tol = attn_tol(ref, mag, top, 1400, 64, pieces(q_dtype, out_dtype), out_dtype)
+    assert bool(((got[:, None] - ref).abs() <= tol).all())
+
+
+def test_captured_with_scales_far_apart():
+    c, k, v = filled(3, 2, 700, 64, seed=15)
+    raised(c, (slice(None), 0, 5), 50)
+    q, lens = torch.randn(3, 4, 64, device="cuda"), i32([700, 3, 90])
+    c.decode(q, lens)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = c.decode(q, lens, dtype=torch.float32)
+    for i in range(4):
+        q.copy_(torch.randn(3, 4, 64))
+        c.v_scale[1, :, 1 + i] ^= 64  # some keys 2^64 larger or smaller than before
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, c.decode(q, lens, dtype=torch.float32)) and torch.isfinite(y).all(), i
