@@ -528,10 +528,11 @@ int itts_fp8_quant_rows(const void* x, int64_t ldx, int x_dtype, int64_t M, int 
                         int64_t lds, void* stream);
 /* y [M][N] = act(Q(x) Q(w)^T + bias) + residual: x [M][K] f32 or bf16 is quantised within the call, w comes
  * quantised (itts_fp8_quant_rows), bias [N] f32 and residual [M][ldr] f32 optional (residual may be y itself; y must
- * not overlap x), act 0 none, 1 gelu_tanh, 2 SiLU (as itts_igemm_fwd), y f32 (exact products, f32 accumulation) or bf16 (the 8-bit
- * matrix unit: f32 accumulation of 128 products at a time, which it aligns to the largest of them).  A row's result does
- * not depend on the other rows' values; workspace: itts_fp8_linear_workspace_bytes (0: none needed), 16-B aligned,
- * not shared by calls that may run at the same time (two captured graphs included). */
+ * not overlap x, nor residual otherwise), act 0 none, 1 gelu_tanh, 2 SiLU (as itts_igemm_fwd), y f32 (exact products,
+ * f32 accumulation) or bf16 (the 8-bit matrix unit: f32 accumulation of 128 products at a time, which it aligns to the
+ * largest of them).  A row's result does not depend on the other rows' values; workspace:
+ * itts_fp8_linear_workspace_bytes (0: none needed), 16-B aligned, not shared by calls that may run at the same time (two
+ * captured graphs included). */
 int64_t itts_fp8_linear_workspace_bytes(int64_t M, int N, int K);
 int itts_fp8_linear(const void* x, int64_t ldx, int x_dtype, int64_t M, int K, const uint8_t* wq, int64_t ldw,
                     const uint8_t* ws, int64_t ldws, int N, const float* bias, int act, const float* residual,

@@ -78,7 +78,7 @@ class Fp8Linear:
     def __call__(self, x: torch.Tensor, act: int = 0, residual: Optional[torch.Tensor] = None, bf16_out: bool = False,
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """act(x @ W^T + b) (+ residual); act 0 none, 1 gelu_tanh, 2 SiLU; y f32, or bf16 with ``bf16_out``;
-        residual f32 [..., N], contiguous, may be ``out`` itself; ``out`` must not overlap x."""
+        residual f32 [..., N], contiguous, may be ``out`` itself; ``out`` must not overlap x, nor residual otherwise."""
         K, N, dev = self.in_features, self.out_features, self.index
         shape = x.shape
         xd = _CODE.get(x.dtype)
@@ -108,6 +108,9 @@ class Fp8Linear:
                     residual.get_device() != dev:
                 raise ValueError(f"residual must be a contiguous f32 tensor of {ys} on {self.dev}")
             res = residual.data_ptr()
+            if out is not None and M and (res != y.data_ptr() or bf16_out):  # out itself: each value is read where it is written
+                if res < y.data_ptr() + M * N * y.element_size() and y.data_ptr() < res + M * N * 4:
+                    raise ValueError("residual must be out itself or not overlap it")
         if M == 0:
             return y
         n = _workspace_bytes(M, N, K)

@@ -161,3 +161,17 @@ def test_captured_with_scales_far_apart():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, c.decode(q, lens, dtype=torch.float32)) and torch.isfinite(y).all(), i
+
+
+def test_a_residual_that_overlaps_out_is_refused():
+    from indextts.utils.fp8 import Fp8Linear
+    layer = Fp8Linear.from_weight(torch.randn(64, 128, device="cuda"))
+    x, both = torch.randn(40, 128, device="cuda"), torch.randn(81, 64, device="cuda")
+    for res, out in ((both[:40], both[1:41]), (both[1:41], both[:40]), (both[39:79], both[:40])):
+        with pytest.raises(ValueError):
+            layer(x, residual=res, out=out)
+    with pytest.raises(ValueError):
+        layer(x, residual=both[:40], out=both[:20].view(torch.bfloat16).view(40, 64), bf16_out=True)
+    want = layer(x, residual=both[41:])
+    assert torch.equal(layer(x, residual=both[41:], out=both[:40]), want)
+    assert torch.equal(layer(x, residual=both[41:], out=both[41:]), want)
