@@ -568,7 +568,8 @@ int64_t itts_attn_cached_workspace_bytes(const ItTsKvCache* c, int B, int T, int
  * itts_attn_decode_rows; ld_rows 0: one table for all rows); an entry outside the cache makes that row's output NaN.
  * kv_len outside 0 .. max_kv: NaN.
  * max_len: the largest kv_len the caller expects (it sizes the split over keys; larger ones stay right).
- * q f32 or bf16, out bf16 or f32 (strides in elements, unit head_dim stride); out must not overlap q or the cache. */
+ * q f32 or bf16, out bf16 or f32 (strides in elements, unit head_dim stride); out may be q itself (type and strides
+ * alike); it must not overlap q otherwise, nor the cache. */
 int itts_attn_decode_kv8(const ItTsKvCache* c, const void* q, int64_t q_sb, int64_t q_sh, int q_dtype, int B, int group,
                          const int32_t* kv_len, const int32_t* pad, const int32_t* kv_rows, int64_t ld_rows, float scale,
                          int max_len, void* out, int64_t o_sb, int64_t o_sh, int out_dtype, void* workspace, void* stream);

@@ -273,7 +273,8 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
   };
   load_first();
 
-  // this lane's columns, their masks and Q
+  // this lane's columns, their masks and Q.  No other workgroup takes these columns, and all four waves have read them before the
+  // first barrier: the result may lie where Q is.
   int col[NQ], tok[NQ];
   uint64_t msk[NQ];
   u32x4_t qf[NQ][KS][QN];

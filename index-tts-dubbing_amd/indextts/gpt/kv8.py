@@ -12,6 +12,7 @@ and every argument that changes from step to step lives on the device, so calls 
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -19,6 +20,49 @@ import torch
 from .. import _hip
 
 _CODE = {torch.float32: _hip.F32, torch.bfloat16: _hip.BF16}
+
+
+# Where tensors with unit last stride lie in memory.  A layout is (shape, strides, bytes of an element); its pieces are the runs of the
+# last dim.  Layouts repeat from call to call, so what is worked out for them is kept.
+
+@lru_cache(4096)
+def _extent(shape, strides, size) -> int:
+    """bytes from the first element to behind the last"""
+    return size * (1 + sum((n - 1) * s for n, s in zip(shape, strides))) if 0 not in shape else 0
+
+
+def _pieces(shape, strides, size) -> torch.Tensor:
+    at = torch.zeros(1, dtype=torch.int64)
+    for n, s in zip(shape[:-1], strides[:-1]):
+        at = (at[:, None] + torch.arange(n) * (s * size)).reshape(-1)
+    return at.sort().values
+
+
+@lru_cache(4096)
+def _distinct(shape, strides, size) -> bool:
+    """whether no two elements share memory"""
+    dims = sorted((s, n) for n, s in zip(shape[:-1], strides[:-1]) if n > 1)
+    span = shape[-1]
+    for s, n in dims:  # each dim steps over the ones within it: the usual case
+        if s < span:
+            at = _pieces(shape, strides, size)
+            return bool((at[1:] - at[:-1] >= shape[-1] * size).all())
+        span += (n - 1) * s
+    return True
+
+
+@lru_cache(4096)
+def _out_extent(shape, strides, size) -> int:
+    """_extent (1 for an empty tensor), 0 where elements share memory"""
+    return max(_extent(shape, strides, size), 1) if _distinct(shape, strides, size) else 0
+
+
+@lru_cache(4096)
+def _meet(a, b, offset) -> bool:
+    """whether layouts a and b share memory, b's first element ``offset`` bytes behind a's"""
+    pa, pb = _pieces(*a), _pieces(*b) + offset
+    la, lb = a[0][-1] * a[2], b[0][-1] * b[2]
+    return bool((torch.searchsorted(pb, pa + la) > torch.searchsorted(pb, pa - lb, right=True)).any())
 
 
 class _Cache:
@@ -52,6 +96,11 @@ class _Cache:
         self.scale = hd ** -0.5
         self.lib = _hip.load()
         self._need = {}  # workspace bytes by the sizes of a call
+        self._held = []  # (first byte, last + 1, layout) of the cache's tensors; a head's positions are one piece
+        for t in (k, v) if k_scale is None else (k, v, k_scale, v_scale):
+            layout = ((rows, heads, t[0, 0].numel()), (t.stride(0), t.stride(1), 1), t.element_size())
+            self._held.append((t.data_ptr(), t.data_ptr() + _extent(*layout), layout))
+        self._first, self._end = min(t[0] for t in self._held), max(t[1] for t in self._held)
 
     def _index(self, t: Optional[torch.Tensor], n: int, name: str) -> Optional[int]:
         if t is None:
@@ -82,6 +131,23 @@ class _Cache:
                              f"last stride on {self.dev}, got {tuple(shape)} {t.dtype}")
         return group
 
+    def _check_out(self, out: torch.Tensor, q: torch.Tensor, os, qs) -> None:
+        """out over itself, over q (unless it is q: a column's q is read before its result is written) or over the cache"""
+        shape, lo, at, size = out.shape, out.data_ptr(), q.data_ptr(), out.element_size()
+        extent = _out_extent(shape, os, size)
+        if not extent:
+            raise ValueError("out holds the same memory twice")
+        hi = lo + extent
+        if at < hi and (at != lo or os != qs or q.dtype != out.dtype):
+            layout = (shape, qs, q.element_size())
+            same = at == lo and q.dtype == out.dtype and all(n == 1 or s == t for n, s, t in zip(shape, os, qs))
+            if not same and lo < at + _extent(*layout) and _meet((shape, os, size), layout, at - lo):
+                raise ValueError("out must be q itself or not overlap it")
+        if lo < self._end and self._first < hi:
+            for first, end, held in self._held:
+                if first < hi and lo < end and _meet((shape, os, size), held, first - lo):
+                    raise ValueError("out must not overlap the cache")
+
     def _workspace(self, B, T, group, max_len, q_dtype):
         n = self._need.get((B, T, group, max_len, q_dtype))
         if n is None:
@@ -100,7 +166,8 @@ class _Cache:
         each row's kv_len [B] accepted positions (drafted token j at position kv_len[b] + j).  mask [B, T] int64 (or [T]:
         one tree for all rows): bit j of mask[b, t] lets token t see drafted token j; every token also sees the row's
         positions pad[b] .. kv_len[b] - 1.  n_tokens [B]: drafted tokens of each row (all T if None); the outputs of the
-        others stay as they are in ``out`` (zero without one).  ``tree_mask`` makes masks from parents."""
+        others stay as they are in ``out`` (zero without one).  ``out`` may be q itself; it must not overlap q otherwise, nor
+        the cache.  ``tree_mask`` makes masks from parents."""
         shape = q.shape
         if len(shape) != 4:
             raise ValueError(f"q must be [B, T, heads, head_dim], got {tuple(shape)}")
@@ -110,17 +177,21 @@ class _Cache:
         if mask.dtype != torch.int64 or mask.shape != ((T,) if one else (B, T)) or mask.stride(-1) != 1 and T > 1 or \
                 mask.get_device() != self.index:
             raise ValueError(f"mask must be int64 [{B}, {T}] or [{T}] with unit last stride on {self.dev}")
+        qs = q.stride()
         if out is None:
             out = torch.zeros(shape, dtype=dtype, device=self.dev)
-        elif out.shape != shape or out.stride(3) != 1 or out.get_device() != self.index:
-            raise ValueError(f"out must be {tuple(shape)} with unit last stride on {self.dev}")
+            os = out.stride()
+        else:
+            os = out.stride()
+            if out.shape != shape or os[3] != 1 or out.get_device() != self.index:
+                raise ValueError(f"out must be {tuple(shape)} with unit last stride on {self.dev}")
+            self._check_out(out, q, os, qs)
         qd, od = _CODE[q.dtype], _CODE.get(out.dtype)
         if od is None or od == _hip.F32 and self._c.dtype == _hip.BF16:
             raise ValueError("out must be bf16, or f32 over an 8-bit cache")
         rows, ld = self._lineage(kv_rows, B)
         longest = self.max_kv if max_len is None else int(max_len)
         ws = self._workspace(B, T, group, longest, qd)
-        qs, os = q.stride(), out.stride()
         rc = self.lib.itts_attn_tree(
             self._ref, q.data_ptr(), qs[0], qs[1], qs[2], qd, B, T, group, self._index(kv_len, B, "kv_len"),
             self._index(pad, B, "pad"), self._index(n_tokens, B, "n_tokens"), mask.data_ptr(), 0 if one else mask.stride(0),
@@ -184,25 +255,29 @@ class Kv8Cache(_Cache):
                kv_rows: Optional[torch.Tensor] = None, max_len: Optional[int] = None, scale: Optional[float] = None,
                out: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """Single-token attention: q [B, heads * group, head_dim] over positions pad[b] .. kv_len[b] - 1 of each row
-        (this step's K/V written before); scale defaults to head_dim ** -0.5; out bf16 or f32 like q.  kv_rows
-        [B, >= max_kv] int32: the cache row that holds each position (beams; one table may be expanded over the rows).
-        max_len: the largest kv_len expected (the split over keys is sized by it; default max_kv)."""
+        (this step's K/V written before); scale defaults to head_dim ** -0.5; out bf16 or f32, q itself or apart
+        from q and the cache.  kv_rows [B, >= max_kv] int32: the cache row that holds each position (beams; one table
+        may be expanded over the rows).  max_len: the largest kv_len expected (the split over keys is sized by it;
+        default max_kv)."""
         shape = q.shape
         if len(shape) != 3:
             raise ValueError(f"q must be [B, heads, head_dim], got {tuple(shape)}")
         group = self._heads(q, shape, "q")
-        B = shape[0]
+        B, qs = shape[0], q.stride()
         if out is None:
             out = q.new_empty(shape, dtype=dtype)
-        elif out.shape != shape or out.stride(2) != 1 or out.get_device() != self.index:
-            raise ValueError(f"out must be {tuple(shape)} with unit last stride on {self.dev}")
+            os = out.stride()
+        else:
+            os = out.stride()
+            if out.shape != shape or os[2] != 1 or out.get_device() != self.index:
+                raise ValueError(f"out must be {tuple(shape)} with unit last stride on {self.dev}")
+            self._check_out(out, q, os, qs)
         qd, od = _CODE[q.dtype], _CODE.get(out.dtype)
         if od is None:
             raise ValueError("out must be f32 or bf16")
         rows, ld = self._lineage(kv_rows, B)
         longest = self.max_kv if max_len is None else int(max_len)
         ws = self._workspace(B, 1, group, longest, qd)
-        qs, os = q.stride(), out.stride()
         rc = self.lib.itts_attn_decode_kv8(
             self._ref, q.data_ptr(), qs[0], qs[1], qd, B, group, self._index(kv_len, B, "kv_len"), self._index(pad, B, "pad"),
             rows, ld, self.scale if scale is None else float(scale), longest, out.data_ptr(), os[0], os[1], od,

@@ -48,3 +48,46 @@ def test_rows_fetched_for_a_tile_of_weights_lie_within_them(tmp_path):
         j, r = i >> 4 & 3, i & 15
         assert rows[255, i] == (i & 192) + 16 * (r // 4) + 4 * j + r % 4
     assert torch.equal(rows, torch.minimum(rows[255][None], torch.arange(256)[:, None]))  # never behind the last
+
+
+def test_where_an_output_may_lie():
+    """out beside, over and between q and the cache: exact to the element, also for layouts that interleave"""
+    from indextts.gpt.kv8 import _Cache, _distinct, _extent, _meet
+    base = torch.zeros(1 << 16, dtype=torch.uint8)
+
+    def places(layout, at):
+        el = [0]
+        for n, s in zip(layout[0], layout[1]):
+            el = [e + i * s for e in el for i in range(n)]
+        return [at + e * layout[2] + b for e in el for b in range(layout[2])]
+
+    g = torch.Generator().manual_seed(0)
+    for _ in range(300):
+        def one():
+            shape = tuple(int(v) for v in torch.randint(1, 4, (3,), generator=g)) + (4,)
+            return shape, tuple(int(v) for v in torch.randint(0, 40, (3,), generator=g)) + (1,), 2 + 2 * int(torch.randint(2, (1,), generator=g))
+        a, b, off = one(), one(), 2 * int(torch.randint(-100, 100, (1,), generator=g))
+        pa, pb = places(a, 0), places(b, off)
+        assert _meet(a, b, off) == bool(set(pa) & set(pb))
+        assert _distinct(*a) == (len(set(pa)) == len(pa))
+        assert _extent(*a) == max(pa) + 1
+
+    c = object.__new__(_Cache)
+    c.index, c.dev = -1, torch.device("cpu")
+    cache = base[8192:8192 + 2 * 2 * 16 * 64].view(2, 2, 16, 64)
+    layout = ((2, 2, 16 * 64), (2 * 16 * 64, 16 * 64, 1), 1)
+    c._first, c._end = cache.data_ptr(), cache.data_ptr() + cache.numel()
+    c._held = [(c._first, c._end, layout)]
+    qkv = base[16384:16384 + 3 * 3 * 2 * 64 * 4].view(torch.float32).view(3, 3, 2, 64)
+    q = qkv[:, 0]
+    for out in (q, qkv[:, 1], qkv[:, 2], q.view(3, 1, 2, 64).squeeze(1), torch.zeros(3, 2, 64), torch.zeros(3, 2, 64, dtype=torch.bfloat16),
+                base[:768].view(torch.bfloat16).view(3, 2, 64)):
+        c._check_out(out, q, out.stride(), q.stride())
+    c._check_out(q[:0], q[:0], q.stride(), q.stride())
+    flat = qkv.view(-1)
+    for out in (flat.as_strided((3, 2, 64), (384, 64, 1), q.storage_offset() + 1),
+                flat.as_strided((3, 2, 64), (128, 64, 1), q.storage_offset()),  # rows 1, 2 over q's row 0 .. k
+                q.view(torch.bfloat16)[..., :64], q[:1].expand(3, 2, 64), q[:, :1].expand(3, 2, 64),
+                cache.view(-1)[64:64 + 768].view(torch.bfloat16).view(3, 2, 64)):
+        with pytest.raises(ValueError):
+            c._check_out(out, q, out.stride(), q.stride())

@@ -175,3 +175,25 @@ def test_a_residual_that_overlaps_out_is_refused():
     want = layer(x, residual=both[41:])
     assert torch.equal(layer(x, residual=both[41:], out=both[:40]), want)
     assert torch.equal(layer(x, residual=both[41:], out=both[41:]), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("longest", [60, 3000])
+def test_out_may_be_q(dtype, longest):
+    """in one part and split over the keys; more columns than one workgroup takes; also out between q's rows"""
+    c, _, _ = filled(3, 2, 3000, 64, seed=21)
+    g = torch.Generator().manual_seed(22)
+    lens = i32([60, 0, 33]) if longest == 60 else i32([2900, 7, 1100])
+    qkv = torch.randn(3, 3, 2 * 20, 64, generator=g).to(dtype).cuda()
+    q = qkv[:, 0]
+    want = c.decode(q, lens, max_len=longest, dtype=dtype)
+    assert torch.equal(c.decode(q, lens, max_len=longest, out=qkv[:, 1]), want)
+    assert c.decode(q, lens, max_len=longest, out=q) is q and torch.equal(q, want)
+    q = torch.randn(3, 33, 4, 64, generator=g).to(dtype).cuda()
+    mask = torch.arange(1, 34, device="cuda")
+    want = c.tree(q, lens, mask, max_len=longest, dtype=dtype)
+    assert torch.equal(c.tree(q, lens, mask, max_len=longest, out=q), want)
+    for out in (qkv[:, 0, :, :].as_strided((3, 40, 64), qkv[:, 0].stride(), 64), c.k.view(-1)[:3 * 40 * 64 * 4].view(torch.float32).view(3, 40, 64),
+                qkv[:, 0, :1].expand(3, 40, 64)):
+        with pytest.raises(ValueError):
+            c.decode(qkv[:, 0], lens, out=out)
