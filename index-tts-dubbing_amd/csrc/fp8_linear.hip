@@ -461,7 +461,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const T* p, int64_t 
 
 // The 256 accumulator registers of a wave are all sums.  As a builtin the compiler moves a third of them on every turn of the
 // loop and spills; as assembly they stay.  A sum is next touched 64 products later, operands come from the LDS (the
-// compiler waits for those), and what the vector unit writes or reads next to a product is kept apart by s_nop.
+// compiler waits for those), and what the vector unit writes or reads next to a product is kept apart by s_nop.  That the compiler
+// adds no vector instruction of its own there -- it knows of no wait that these products need -- is checked in the assembly when this
+// file is built.  (An s_nop before every product would do as well: 8192 x 8192 x 8192 443 -> 451 us.)
 template <int S>  // which byte of the scale registers
 __device__ __forceinline__ void product_agpr(f32x4_t& acc, const i32x8_t& w, const i32x8_t& x, uint32_t ws, uint32_t xs) {
   if constexpr (S == 0)

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import glob
 import os
+import re
 import shlex
 import subprocess
 import sys
@@ -41,6 +42,63 @@ def needs_rebuild(out: str = OUT) -> bool:
     return any(os.path.getmtime(s) > t for s in sources() + _headers())
 
 
+# ---- matrix products written as inline assembly (csrc/fp8_linear.hip) ----
+# The compiler does not know them as matrix instructions, so it puts no waits between a vector instruction that writes an operand and
+# the product, nor around a copy of the sums, which it may place anywhere.  That the kernel holds neither is a property of its
+# assembly, looked at whenever the file is compiled.
+CHECKED = {"fp8_linear.hip": "fp8_linear_large_kernel"}
+WAIT = 4  # issue slots between a vector write and the product that reads it (two are needed)
+
+
+def _registers(operand):
+    m = re.fullmatch(r"([va])\[(\d+):(\d+)\]", operand)
+    if m:
+        return {m[1] + str(i) for i in range(int(m[2]), int(m[3]) + 1)}
+    return {operand} if re.fullmatch(r"[va]\d+", operand) else set()
+
+
+def check_products(text: str, kernel: str) -> int:
+    """The number of products in the functions of the assembly whose name holds ``kernel``; RuntimeError where one may read a
+    vector register too early, or where anything but a product touches a sum between the first and the last."""
+    count = 0
+    for name, body in re.findall(r"^(\w*%s\w*):(.*?)^\.Lfunc_end" % kernel, text, re.M | re.S):
+        code, label, jumps = [], {}, {}  # instructions as (name, operands); label -> index of the next one, and of jumps to it
+        for line in body.split("\n"):
+            line = line.split(";")[0].strip()
+            if line.startswith(".LBB"):
+                label[line.rstrip(":")] = len(code)
+            elif line and not line.startswith("."):
+                op, _, rest = line.partition(" ") if " " in line else line.partition("\t")
+                operands = [o.strip().split(" ")[0] for o in rest.split(",")]
+                if op.startswith(("s_cbranch", "s_branch")):
+                    jumps.setdefault(operands[0], []).append(len(code))
+                code.append((op, operands))
+        into = {}
+        for at, froms in ((label[k], v) for k, v in jumps.items()):
+            into.setdefault(at, []).extend(froms)
+        products = [i for i, (op, _) in enumerate(code) if op.startswith("v_mfma")]
+        count += len(products)
+        for i in products:
+            reads = set().union(*(_registers(o) for o in code[i][1][1:]))
+            todo, seen = [(i, WAIT)], set()
+            while todo:
+                at, left = todo.pop()
+                if left <= 0 or (at, left) in seen:
+                    continue
+                seen.add((at, left))
+                todo += [(j, left - 1) for j in into.get(at, ())]
+                if at == 0 or code[at - 1][0] in ("s_branch", "s_endpgm"):
+                    continue
+                op, operands = code[at - 1]
+                if op.startswith("v_") and not op.startswith("v_mfma") and _registers(operands[0]) & reads:
+                    raise RuntimeError(f"{name}: {op} {', '.join(operands)} right before the product that reads it")
+                todo.append((at - 1, left - (1 + int(operands[0], 0) if op == "s_nop" else 1)))
+        for op, operands in code[products[0]:products[-1]] if products else ():
+            if not op.startswith("v_mfma") and any(r[0] == "a" for o in operands for r in _registers(o)):
+                raise RuntimeError(f"{name}: {op} {', '.join(operands)} among the products")
+    return count
+
+
 def build(force: bool = False, verbose: bool = True, out: str = None) -> str:
     out = out or os.environ.get("ITTS_BUILD_OUT", OUT)
     defs = shlex.split(os.environ.get("ITTS_HIPCC_DEFS", ""))
@@ -60,6 +118,12 @@ def build(force: bool = False, verbose: bool = True, out: str = None) -> str:
         if verbose:
             print("[itts build]", os.path.basename(src), " ".join(defs), flush=True)
         subprocess.run(cmd, check=True)
+        kernel = CHECKED.get(os.path.basename(src))
+        if kernel:
+            subprocess.run([*cmd[:cmd.index("-c")], "--cuda-device-only", "-S", src, "-o", obj + ".s"], check=True)
+            with open(obj + ".s") as f:
+                if not check_products(f.read(), kernel):
+                    raise RuntimeError(f"no products of {kernel} in the assembly of {src}")
         os.replace(obj + ".tmp", obj)
         return obj
 

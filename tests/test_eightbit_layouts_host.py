@@ -91,3 +91,36 @@ def test_where_an_output_may_lie():
                 cache.view(-1)[64:64 + 768].view(torch.bfloat16).view(3, 2, 64)):
         with pytest.raises(ValueError):
             c._check_out(out, q, out.stride(), q.stride())
+
+
+def test_the_check_of_the_assembly_products():
+    """what _build looks for in the assembly of the products written by hand, on a loop of two of them"""
+    from indextts._build import check_products
+    good = """_Z5largev:
+	v_mov_b32_e32 v40, v41
+	s_nop 7
+.LBB0_1:                                ; =>This Inner Loop Header: Depth=1
+	ds_read_b128 v[8:11], v50
+	s_waitcnt lgkmcnt(0)
+	v_mfma_scale_f32_16x16x128_f8f6f4 a[0:3], v[0:7], v[8:15], a[0:3], v40, v42 op_sel_hi:[0,0,0]
+	v_add_u32_e32 v60, v61, v62
+	v_mfma_scale_f32_16x16x128_f8f6f4 a[4:7], v[16:23], v[8:15], a[4:7], v40, v42 op_sel_hi:[0,0,0]
+	s_add_i32 s4, s4, 1
+	s_cbranch_scc1 .LBB0_1
+	v_accvgpr_read_b32 v0, a0
+	s_endpgm
+.Lfunc_end0:
+"""
+    assert check_products(good, "large") == 2 and check_products(good, "other") == 0
+    for old, new in (("	v_add_u32_e32 v60, v61, v62", "	v_add_u32_e32 v60, v61, v62\n	v_mov_b32_e32 v17, v62"),
+                     ("	s_nop 7\n", ""),
+                     ("	s_nop 7\n", "	s_nop 0\n"),
+                     ("	s_add_i32 s4, s4, 1", "	v_mov_b32_e32 v42, v43"),  # reaches the first product over the jump
+                     ("	v_add_u32_e32 v60, v61, v62", "	v_accvgpr_mov_b32 a9, a0"),
+                     ("	v_add_u32_e32 v60, v61, v62", "	v_accvgpr_read_b32 v60, a2"),
+                     ("	s_waitcnt lgkmcnt(0)", "	v_lshlrev_b32_e32 v12, 8, v13")):
+        bad = good.replace(old, new)
+        assert bad != good
+        with pytest.raises(RuntimeError):
+            check_products(bad, "large")
+    assert check_products(good.replace("	s_add_i32 s4, s4, 1", "	v_mov_b32_e32 v42, v43\n	s_nop 3"), "large") == 2
