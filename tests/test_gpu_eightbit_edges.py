@@ -197,3 +197,33 @@ def test_out_may_be_q(dtype, longest):
                 qkv[:, 0, :1].expand(3, 40, 64)):
         with pytest.raises(ValueError):
             c.decode(qkv[:, 0], lens, out=out)
+
+
+@pytest.mark.parametrize("scale", [-0.125, 0.0])
+@pytest.mark.parametrize("e4m3", [True, False])
+def test_scales_that_are_not_positive(scale, e4m3):
+    lens = [0, 5, 200]
+    c, k, v, q, mask = tree_case(3, 6, 2, 2, 64, lens, 33, e4m3, torch.float32)
+    got = c.tree(q, i32(lens), mask, scale=scale)
+    ref = q * (0.0 if scale == 0 else -1.0)  # the same scores at a positive scale
+    check_rows(got, ref, k, v, seen_keys(3, 6, k.shape[2], i32(lens), None, mask), 0.125, pieces(None, torch.bfloat16, e4m3), torch.bfloat16)
+
+
+@pytest.mark.parametrize("apart", [0, 30])
+@pytest.mark.parametrize("longest", [64, 2000])
+def test_stale_slots_and_nan_beside_scales_far_apart(apart, longest):
+    """what is not seen does not reach a result: slots behind the row and before its padding with any byte as scale, and a drafted NaN"""
+    lens = [20, 64]
+    c, k, v, q, mask = tree_case(2, 6, 2, 1, 64, lens, 35, True, torch.float32, smax=90)
+    raised(c, (slice(None), slice(None), 9), apart)
+    pad = i32([3, 40])
+    want = c.tree(q, i32(lens), mask, pad=pad, max_len=longest, dtype=torch.float32)
+    for t, s in ((c.k, c.k_scale), (c.v, c.v_scale)):
+        t[0, :, 26:], t[1, :, 70:], t[0, :, :3] = 0x7F, 0xFF, 0x7E
+        s[0, :, 26:], s[1, :, 70:], s[0, :, :3] = 255, 0, 254
+    assert torch.equal(c.tree(q, i32(lens), mask, pad=pad, max_len=longest, dtype=torch.float32), want)
+    c.v[0, 0, 22, 3], c.v[1, 1, 69, 0] = 0x7F, 0xFF
+    got = c.tree(q, i32(lens), mask, pad=pad, max_len=longest, dtype=torch.float32)
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[0, :, 0, 3], bad[1, :, 1, 0] = (mask[0] >> 2 & 1).bool(), (mask[1] >> 5 & 1).bool()
+    assert torch.equal(torch.isnan(got), bad) and torch.equal(torch.where(bad, 0, got), torch.where(bad, 0, want))
