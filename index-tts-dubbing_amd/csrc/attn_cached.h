@@ -21,11 +21,11 @@
 // (131 keys 5.4 -> 7.0 us; 64 tokens x 4 heads over 16301 keys 110 -> 216).  bf16 V: P as two bf16 parts.
 // Maxima, sums and both products accumulate in f32.
 //
-// What bounds it, and what it takes (kernel time): few tokens over long rows run at the memory's rate (8 rows x 4 heads, up to
-// 32749 keys of 128 dims: 216 MB in 45 us = 4.8 TB/s, and 5 us to join the splits); with lineage tables (96 rows x 16 heads,
-// up to 483 keys of 64 dims) it is the tables' and addresses' arithmetic, 28 us for 78 MB; short rows cost a launch and one
-// trip to memory (131 keys: 5.8 us); many columns (64 tokens x 4 heads, 16301 keys: 116 us for 27 GFLOP, 112 MB) the vector
-// instructions around the products, some 350 per 32 keys and 32 columns, half of them K's and V's conversion.
+// What bounds it, and what it takes (whole calls in a replayed graph): few tokens over long rows run at the memory's rate (8 rows x
+// 4 heads, up to 32749 keys of 128 dims: 216 MB in 45 us = 4.8 TB/s, the join of the splits among them); with lineage tables (96
+// rows x 16 heads, up to 483 keys of 64 dims) it is the tables' and addresses' arithmetic, 29 us for 78 MB; short rows cost a
+// launch and one trip to memory (131 keys: 5.3 us); many columns (64 tokens x 4 heads, 16301 keys: 113 us for 27 GFLOP, 112 MB)
+// the vector instructions around the products, some 250 per 32 keys and 32 columns, half of them for K's and V's conversion.
 #pragma once
 #include <type_traits>
 

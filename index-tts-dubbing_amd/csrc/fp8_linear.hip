@@ -8,9 +8,10 @@
 // f32 outputs: codes times scale are exact in bf16, and v_mfma_f32_16x16x32_bf16 adds exact products to f32 (measured
 // 1.2e-8 of the rms), at half the rate and one conversion per two codes.
 //
-// What bounds it (times with the quantising pass): few rows the launch and the trip to memory (1 x 1024 x 4096: 3.3 us for
-// 4.3 MB, 96 x 4096 x 1024: 8.2); large sizes the matrix unit (8192 x 8192 x 8192: 449 us = 2.45 PFLOP/s) less the tiles' first
-// fetch and last store (14400 x 1024 x 4096 with GELU: 106 us = 1.14 PFLOP/s, four turns of 256 tiles of eight steps each).
+// Times in this file are of whole calls in a replayed graph, the quantising pass included, bf16 results without an activation unless
+// said.  What bounds it: few rows the launch and the trip to memory (1 x 1024 x 4096: 3.4 us for 4.3 MB, 96 x 4096 x 1024: 8.3);
+// large sizes the matrix unit (8192 x 8192 x 8192: 443 us = 2.48 PFLOP/s) less the tiles' first fetch and last store (14400 x 1024 x
+// 4096: 91 us, with GELU 107 = 1.13 PFLOP/s: four turns of 256 tiles of eight steps each).
 #include <type_traits>
 
 #include "fp8.h"
@@ -140,7 +141,7 @@ __device__ __forceinline__ f32x4_t sums_of(f32x4_t a) {
 
 // N a multiple of 16 and aligned rows: a lane has 16 neighbouring results of a row.  They go through the wave's own part of
 // the LDS in their final type, so that neighbouring lanes store neighbouring 16 bytes (stored from where they are, neighbouring
-// lanes on neighbouring rows, a store takes the load / store path 64 clocks instead of 16: XXNOTE).  A row's residual is
+// lanes on neighbouring rows, f32 results of 3500 x 512 x 3600 took 36 us instead of 30).  A row's residual is
 // requested before the stores of the row before (a load waits for the stores before it).
 template <bool BF16, bool AGPR, int ACT, bool RES, int FM, int FN>
 __device__ __forceinline__ void store_direct(const LinearArgs& p, f32x4_t (&acc)[FM][FN], uint8_t* band, int64_t m0, int n0) {
@@ -855,16 +856,16 @@ int64_t code_pitch(int K) { return round_up(K, 128); }
 int64_t scale_pitch(int K) { return round_up(round_up(K, 128) / 128, 4); }
 
 // x quantised within the product (one launch, no workspace) while that is done by few: with more rows or a long k the
-// same values are quantised once per 16 columns of y.  Measured, us (this / quantised first): 1 x 1024 x 4096 3.3 / 5.8,
-// 16 x 4096 x 1024 6.6 / 7.7, 32 x 1024 x 4096 5.5 / 5.8, 32 x 2048 x 1024 6.9 / 6.2, 32 x 4096 x 1024 10.8 / 7.7.
+// same values are quantised once per 16 columns of y.  Measured, us (this / quantised first): 1 x 1024 x 4096 3.4 / 5.0,
+// 16 x 4096 x 1024 6.7 / 7.3, 32 x 1024 x 4096 5.6 / 5.9, 32 x 2048 x 1024 7.0 / 6.3, 32 x 4096 x 1024 11.0 / 7.9.
 bool few_rows(int64_t M, int K) { return M <= 16 || (M <= 32 && K <= 1024); }
 // 32 x 16 outputs per workgroup with k split among its waves, while that is at most three turns of the 256 CUs: a 128 x 128
 // tile takes 0.8 us per block of k, one after the other.  Measured, us (this / such tiles, both with the quantising pass of
-// 2.5): 96 x 4096 x 1024 8.2 / 29, 96 x 1024 x 4096 10.0 / 12.2, 300 x 1024 x 1024 10.0 / 12.4, 800 x 256 x 2048 25 / 8.7.
+// 2.5): 96 x 4096 x 1024 8.3 / 29, 96 x 1024 x 4096 10.0 / 12.3, 300 x 1024 x 1024 10.2 / 12.4, 800 x 256 x 2048 25 / 8.5.
 bool some_rows(int64_t M, int N) { return ((M + 31) / 32) * ((N + 15) / 16) <= 768; }
 // 256 x 256 tiles once they keep most of the 256 CUs busy (and the scales of all of k fit the LDS beside them).  Measured,
-// us with the quantising pass (these / 128 x 128): 14400 x 1024 x 4096 93 / 114, 14400 x 4096 x 1024 84 / 102, 8192 x 8192 x
-// 8192 449 / 644, 3000 x 1024 x 4096 (192 tiles) 27 / 30, 2000 x 1024 x 4096 (128 tiles) 25 / 21.
+// us with the quantising pass (these / 128 x 128): 14400 x 1024 x 4096 91 / 102, with GELU 107 / 115, 14400 x 4096 x 1024 82 / 101,
+// 8192 x 8192 x 8192 443 / 646, 3000 x 1024 x 4096 (192 tiles) 26 / 30, 2000 x 1024 x 4096 (128 tiles) 24 / 20.
 bool large_tiles(int64_t M, int N, int K) {
   return M > 128 && N > 128 && ((M + 255) / 256) * ((N + 255) / 256) >= 160 && K <= 128 * kScaleBlocks;
 }
