@@ -14,17 +14,17 @@
 // Types: e4m3 K times its scale is exact in bf16 (any exponent), so q enters as bf16 and is exact when it is bf16; an f32
 // q enters as three bf16 parts (24 bits).  While the scales of a wave's V keep within a factor 2^12 of each other, e4m3 V is
 // exact in f16 relative to the largest, and P enters as f16 in [0, 2^15] (half step 2^-12 of a weight, below the bf16 output's
-// 2^-9) or, for f32 outputs, as two f16 parts (2^-23); weights below some 2^-21 of the largest keep fewer bits, those below 2^-32
-// none.  Where the scales lie further apart -- in a drafted token that other columns do not see, or in keys without
+// 2^-9) or, for f32 outputs, as two f16 parts (2^-23); of weights below 2^-27 (two parts: 2^-16) of the largest fewer bits are left,
+// down to 2^-38.  Where the scales lie further apart -- in a drafted token that other columns do not see, or in keys without
 // weight -- the wave takes its tiles once more with V as bf16, which is exact with any scale, and P as two bf16 parts (2^-17) or three
 // for f32 outputs: every finite V counts where it is seen and nowhere else.  That costs the second walk: 1.3 to 2 times the time
-// (131 keys 5.4 -> 7.0 us; 64 tokens x 4 heads over 16301 keys 110 -> 216).  bf16 V: P as two bf16 parts.
+// (131 keys 5.3 -> 7.0 us; 64 tokens x 4 heads over 16301 keys 116 -> 220).  bf16 V: P as two bf16 parts.
 // Maxima, sums and both products accumulate in f32.
 //
 // What bounds it, and what it takes (whole calls in a replayed graph): few tokens over long rows run at the memory's rate (8 rows x
 // 4 heads, up to 32749 keys of 128 dims: 216 MB in 45 us = 4.8 TB/s, the join of the splits among them); with lineage tables (96
 // rows x 16 heads, up to 483 keys of 64 dims) it is the tables' and addresses' arithmetic, 29 us for 78 MB; short rows cost a
-// launch and one trip to memory (131 keys: 5.3 us); many columns (64 tokens x 4 heads, 16301 keys: 113 us for 27 GFLOP, 112 MB)
+// launch and one trip to memory (131 keys: 5.3 us); many columns (64 tokens x 4 heads, 16301 keys: 116 us for 27 GFLOP, 112 MB)
 // the vector instructions around the products, some 250 per 32 keys and 32 columns, half of them for K's and V's conversion.
 #pragma once
 #include <type_traits>
@@ -57,15 +57,18 @@ struct AttnArgs {
   float *part, *part_ml;  // [unit][split][column][hd], [unit][split][column][maximum, sum of weights relative to it]
 };
 
-// The column's reference follows the running maximum once that is more than a factor 2^kLag ahead.  In f16 P is held times
-// 2^kPUp relative to it, so within 2^15, and V's codes times 2^7 relative to the largest scale: both within f16.
-constexpr int kLag = 8;
+// The column's reference follows the running maximum once that is more than a factor 2^kLag (bf16: 2^kWideLag) ahead.  In f16 P is
+// held times 2^kPUp relative to it, so within 2^15, and V's codes times 2^7 relative to the largest scale: both within f16.  A shorter
+// lag holds smaller weights and rescales O more often (lags of 2^8 / 2^4 / 2^2 / 2^1, us: 64 tokens x 4 heads over 16301 keys 112 / 114
+// / 116 / 119; few columns alike).
+constexpr int kLag = 2;
 constexpr int kPUp = 15 - kLag;
 constexpr int kVUp = 7;
 // In bf16 P has f32's exponents and stays within 1: a sum of P V overflows no sooner than a sum of V.
-constexpr int kWideUp = -kLag;
+constexpr int kWideLag = 8;
+constexpr int kWideUp = -kWideLag;
 // Scales of V within a factor 2^kSpread of each other go through f16: V is exact there up to 2^22, and what f16 loses of a
-// weight (below 2^-32 of the largest) counts for little whatever its V.
+// weight (below 2^-38 of the largest) counts for little whatever its V.
 constexpr int kSpread = 12;
 
 __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
@@ -594,7 +597,7 @@ __global__ __launch_bounds__(64 * kWaves, (waves_per_simd<E4M3, LINEAGE, HD, QN,
       for (int j = 0; j < NQ; ++j) {
         top[j] = max_rows(max2(max2(max2(x[j][0], x[j][1]), max2(x[j][2], x[j][3])),
                                max2(max2(x[j][4], x[j][5]), max2(x[j][6], x[j][7]))) * a.qk_scale);
-        grow |= top[j] > m[j] + kLag;
+        grow |= top[j] > m[j] + (F16 ? kLag : kWideLag);
       }
       if (__any(grow)) {
 #pragma unroll

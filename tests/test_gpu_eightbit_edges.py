@@ -227,3 +227,27 @@ def test_stale_slots_and_nan_beside_scales_far_apart(apart, longest):
     bad = torch.zeros_like(got, dtype=torch.bool)
     bad[0, :, 0, 3], bad[1, :, 1, 0] = (mask[0] >> 2 & 1).bool(), (mask[1] >> 5 & 1).bool()
     assert torch.equal(torch.isnan(got), bad) and torch.equal(torch.where(bad, 0, got), torch.where(bad, 0, want))
+
+
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+def test_many_small_weights_of_larger_v(out_dtype):
+    """one key has a weight of 1, each of 131072 others e^-24 (2^-34.6) and a V 2^12 larger: together two per cent of the result.
+    In f16 a weight is off by at most 2^-38 of the largest in its wave (half of f16's least step at the scale that weights are held
+    at), and the large key's wave takes a fourth of the keys where they are not split."""
+    from indextts.gpt.kv8 import Kv8Cache
+    S, g = 131073, torch.Generator().manual_seed(17)
+    k = torch.zeros(S, 1, 64)
+    k[0, 0, 0] = 24.0
+    v = 0.5 + torch.rand(1, 1, 64, generator=g).repeat(S, 1, 1)
+    v[1:] *= 2.0 ** 12
+    c = Kv8Cache.empty(1, 1, S, 64)
+    c.write(k.cuda(), v.cuda(), torch.zeros(S, dtype=torch.int32, device="cuda"), torch.arange(S, device="cuda").int())
+    k, v = codes64(c.k, c.k_scale), codes64(c.v, c.v_scale)
+    q = torch.zeros(1, 1, 64, device="cuda")
+    q[..., 0] = 1.0
+    ref, mag, top = attend64(q[:, None].double(), k, v, seen_keys(1, 1, S, i32([S])), 1.0)
+    tol = attn_tol(ref, mag, top, 0, 64, pieces(None, out_dtype), out_dtype) + S / 4 * 2.0 ** -38 * v[0, 0].amax(0)
+    small = ref[0, 0, 0] - v[0, 0, 0] / (1 + (S - 1) * torch.exp(torch.tensor(-24.0, dtype=torch.float64)))
+    assert out_dtype == torch.bfloat16 or bool((small / 4 > 4 * tol[0, 0, 0]).all())  # a fourth of that lost would be seen
+    got = c.decode(q, i32([S]), scale=1.0, max_len=1, dtype=out_dtype)
+    assert bool(((got[:, None].double() - ref).abs() <= tol).all()), float(((got[:, None].double() - ref).abs() / tol).max())
